@@ -93,6 +93,63 @@ struct AttnParams {
 void launch_paged_attn_prefill(const AttnParams& p, int num_tiles, int tile_rows, hipStream_t s);
 void launch_paged_attn_decode(const AttnParams& p, int num_seqs, hipStream_t s);
 
+// ---- scaled_cache.hip, scaled_attention.hip ----
+// The scaled 8-bit cache: e4m3 codes in the layouts of the other caches, and per page and kv head one power of
+// two for the keys' codes and one for the values' (scaled_cache.h).
+struct ScaledAppend {
+  const __bf16* qkv;         // [T, qkv_stride]: q heads | k heads | v heads, rows on 16 bytes
+  int64_t qkv_stride;
+  __bf16* q_out;             // [q_rows, Hq, D]
+  uint8_t* k_cache;          // [NB, Hkv, BS, D]
+  uint8_t* v_cache;          // [NB, Hkv, BS/8, D, 8]
+  float* k_scale;            // [NB, Hkv]
+  float* v_scale;
+  const int64_t* positions;  // [T]
+  const int64_t* slots;      // [T] (negative, or outside the cache: no entry)
+  const float* cos_sin;      // [max_pos, D] = cos | sin
+  const __bf16* q_w;         // [D] or nullptr
+  const __bf16* k_w;
+  int T, q_rows, singles;    // rows whose q is written; leading rows that are single tokens of their sequences
+  int Hq, Hkv, BS, num_blocks;
+  int64_t max_pos;
+  float eps;
+  int rope;
+};
+void launch_scaled_append(const ScaledAppend& p, hipStream_t s);
+
+struct ScaledAttn {
+  const __bf16* q;           // [T, Hq, D]
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  __bf16* out;               // [T, Hq, D]
+  const int* block_tables;   // [B, bt_cols], rows bt_stride apart
+  int64_t bt_stride;
+  int bt_cols;
+  const int* seq_lens;       // [B] keys, the new tokens' among them
+  const int* q_start;        // [B + 1] first row of each sequence (decode: nullptr, row b)
+  int Hq, Hkv, G, BS, num_blocks;
+  float scale_log2;
+  int num_parts, part_size;  // decode: partitions of a row's keys (part_size <= kDecodeMaxPart)
+  float* part_m;             // [B, Hkv, parts, G]
+  float* part_l;
+  float* part_o;             // [B, Hkv, parts, G, D]
+  int* tickets;              // as in AttnParams
+  const int* tile_seq;       // prompts: each tile's sequence and first flattened row
+  const int* tile_row;
+  // rows as the projection gave them (prompts, fused decode): normed and rotated by the kernel
+  const __bf16* qkv;
+  int64_t qkv_stride;
+  const int64_t* positions;
+  const float* cos_sin;
+  int64_t max_pos;
+  const __bf16* q_w;
+  float eps;
+};
+void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s);
+void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, hipStream_t s);
+
 // ---- gemm.hip ----
 int gemm_splitk_choice(int M, int N, int K);
 // counters: zero-initialised int32 per-tile tickets (>= tiles) -> split-K partials are

@@ -1,0 +1,464 @@
+// Attention over the scaled 8-bit cache (scaled_cache.h): single rows of running sequences (decode) and rows of
+// prompts.  S^T = K Q^T and O^T = V^T P^T on the matrix cores, keys as rows and queries as columns, so that a
+// query's maximum and sum stay in one lane column; queries and softmax weights are bf16, codes are widened to
+// bf16 with their scale, which is exact, sums and statistics are fp32.
+//
+// A key is seen if it lies inside the sequence's length, the block table and a page of the cache (a table entry
+// outside the cache: its keys are left out).  A row that sees none is zero.
+#include "scaled_cache.h"
+#include "kernels.h"
+
+namespace akap {
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+constexpr int D = 128;
+
+// keys of a sequence that its block table can hold
+__device__ __forceinline__ int keys_of(const ScaledAttn& p, int seq) {
+  const int64_t most = (int64_t)p.bt_cols * p.BS;
+  const int n = p.seq_lens[seq];
+  return n < 0 ? 0 : n < most ? n : (int)most;
+}
+
+// ------------------------------------------------------------------------------------------------- decode
+// grid (sequences, kv heads, partitions), four waves that take a partition's 32-token chunks in turn; the rows of
+// the 16 x 16 x 32 products are the kv head's query heads.  A chunk is 8 loads of 16 bytes to a lane: of K the dims
+// 64 p + 16 g .. + 15 of a token (its k-steps 2 p and 2 p + 1 contract over the first and second 8, q in the same
+// order), of V two dims of an 8-token group.
+struct Chunk {
+  u32x4 k[2][2];   // [16-token tile][p]
+  u32x4 v[4];      // dims 32 n + 2 r and + 1 of group g
+};
+
+__device__ __forceinline__ void chunk_load(Chunk& c, const ScaledAttn& p, int64_t page, int in_page) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const uint8_t* kb = p.k_cache + page + (size_t)in_page * D + (g >> 1) * 512 + r * 32 + (g & 1) * 16;
+  const uint8_t* vb = p.v_cache + page + (size_t)(in_page / 8 + g) * D * 8 + r * 16;
+#pragma unroll
+  for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      c.k[tt][i] = ld_nt(reinterpret_cast<const u32x4*>(kb + tt * 2048 + i * 1024));
+#pragma unroll
+  for (int n = 0; n < 4; ++n) c.v[n] = ld_nt(reinterpret_cast<const u32x4*>(vb + n * 256));
+}
+
+struct Row {
+  f32x4 o[8];      // dims 32 (i >> 1) + 8 g + 2 j + (i & 1), j = 0..3
+  float m, l;      // running maximum (log2), this lane's part of the sum
+};
+
+// END: the chunk holds keys from `end` on that are not seen (and may hold any codes)
+template <bool END>
+__device__ __forceinline__ void chunk_take(Row& st, const bf16x8 (&q)[4], Chunk& c, float kscale, float vscale,
+                                           int left) {
+  const int g = (threadIdx.x & 63) >> 4;
+  f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int tt = 0; tt < 2; ++tt) {
+      s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_wide(c.k[tt][i][0], c.k[tt][i][1], 1.f), q[2 * i], s[tt], 0, 0, 0);
+      s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_wide(c.k[tt][i][2], c.k[tt][i][3], 1.f), q[2 * i + 1], s[tt], 0, 0, 0);
+    }
+  float x[8], top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {      // token 8 g + i of the chunk
+    x[i] = s[i >> 2][i & 3] * kscale;
+    if (END && 8 * g + i >= left) x[i] = -INFINITY;
+    top = fmaxf(top, x[i]);
+  }
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  const float m = fmaxf(st.m, top), a = __builtin_amdgcn_exp2f(st.m - m);
+  st.m = m;
+  float sum = 0.f;
+  bf16x8 w;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float e = __builtin_amdgcn_exp2f(x[i] - m);
+    sum += e;
+    w[i] = f2bf(e);
+  }
+  st.l = st.l * a + sum;
+  if (END) {                         // what lies behind the end may be no number: zeros
+    const int mine = left - 8 * g;
+    const uint32_t lo = mine >= 4 ? ~0u : mine <= 0 ? 0u : (1u << (8 * mine)) - 1;
+    const uint32_t hi = mine >= 8 ? ~0u : mine <= 4 ? 0u : (1u << (8 * (mine - 4))) - 1;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) c.v[n] = u32x4{c.v[n][0] & lo, c.v[n][1] & hi, c.v[n][2] & lo, c.v[n][3] & hi};
+  }
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      f32x4& o = st.o[2 * n + e];
+      o *= a;
+      o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_wide(c.v[n][2 * e], c.v[n][2 * e + 1], vscale), w, o, 0, 0, 0);
+    }
+}
+
+// The partitions of a (sequence, kv head): 16 threads to a row, 8 dims to a thread.
+__device__ __forceinline__ void merge(const ScaledAttn& p, int seq, int kvh, int nparts, int q_tok) {
+  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  if (row >= p.G) return;
+  const size_t base = (size_t)(seq * p.Hkv + kvh) * p.num_parts * p.G + row;
+  float M = -1e30f, L = 0.f, acc[8] = {};
+  for (int i = 0; i < nparts; ++i) M = fmaxf(M, p.part_m[base + (size_t)i * p.G]);
+  for (int i = 0; i < nparts; ++i) {
+    const size_t at = base + (size_t)i * p.G;
+    const float f = __builtin_amdgcn_exp2f(p.part_m[at] - M) * p.part_l[at];
+    L += f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += f * p.part_o[at * D + d0 + j];
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  bf16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = f2bf(acc[j] * inv);
+  *reinterpret_cast<bf16x8*>(p.out + ((size_t)q_tok * p.Hq + kvh * p.G + row) * D + d0) = o;
+}
+
+__global__ __launch_bounds__(256) void scaled_merge_kernel(ScaledAttn p) {
+  const int seq = blockIdx.x, keys = keys_of(p, seq);
+  merge(p, seq, blockIdx.y, min(p.num_parts, (keys + p.part_size - 1) / p.part_size), p.q_start ? p.q_start[seq] : seq);
+}
+
+__global__ __launch_bounds__(256, 2) void scaled_decode_kernel(ScaledAttn p) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int seq = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
+  const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = p.G, BS = p.BS;
+  const int first = part * p.part_size, keys = keys_of(p, seq), end = min(keys, first + p.part_size);
+  const int q_tok = p.q_start ? p.q_start[seq] : seq;
+  if (p.num_parts > 1 && first >= keys) return;     // (the merge leaves it out)
+  // page and scales of the wave's chunk `lane` (the host bounds a partition to 64 chunks a wave)
+  const int t0 = first + 32 * w, tok = t0 + 128 * lane;
+  int page = -1;
+  float ks = 0.f, vs = 0.f;
+  if (tok < end) {
+    page = p.block_tables[(size_t)seq * p.bt_stride + tok / BS];
+    if ((uint32_t)page >= (uint32_t)p.num_blocks) page = -1;
+    if (page >= 0) {
+      ks = p.k_scale[(size_t)page * p.Hkv + kvh] * p.scale_log2;
+      vs = p.v_scale[(size_t)page * p.Hkv + kvh];
+    }
+  }
+  bf16x8 q[4];
+  const bf16* qp = p.q + ((size_t)q_tok * p.Hq + kvh * G + min(r, G - 1)) * D + 16 * g;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    q[i] = *reinterpret_cast<const bf16x8*>(qp + 64 * (i >> 1) + 8 * (i & 1));
+    if (r >= G) q[i] = bf16x8{};
+  }
+  Row st;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) st.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  st.m = -1e30f;
+  st.l = 0.f;
+  for (int t = t0, i = 0; t < end; t += 128, ++i) {
+    const int blk = __builtin_amdgcn_readlane(page, i);
+    if (blk < 0) continue;
+    Chunk c;
+    chunk_load(c, p, ((int64_t)blk * p.Hkv + kvh) * BS * D, t % BS);
+    const float ksc = lane_f(ks, i), vsc = lane_f(vs, i);
+    if (t + 32 <= end) chunk_take<false>(st, q, c, ksc, vsc, 32);
+    else chunk_take<true>(st, q, c, ksc, vsc, end - t);
+  }
+  float l = st.l;
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  float* o_s = lds;                               // [4][G][D + 4]
+  float* m_s = lds + 4 * G * (D + 4);             // [4][G]
+  float* l_s = m_s + 4 * G;
+  if (r < G) {
+    float* to = o_s + (w * G + r) * (D + 4) + 8 * g;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x2*>(to + 32 * n + 2 * j) = f32x2{st.o[2 * n][j], st.o[2 * n + 1][j]};
+    if (g == 0) {
+      m_s[w * G + r] = st.m;
+      l_s[w * G + r] = l;
+    }
+  }
+  __syncthreads();
+  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
+  if (row >= G) return;
+  float M = -1e30f, L = 0.f, acc[8] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i * G + row]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float f = __builtin_amdgcn_exp2f(m_s[i * G + row] - M);
+    L += f * l_s[i * G + row];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] += f * o_s[(i * G + row) * (D + 4) + d0 + j];
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  if (p.num_parts == 1) {
+    bf16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = f2bf(acc[j] * inv);
+    *reinterpret_cast<bf16x8*>(p.out + ((size_t)q_tok * p.Hq + kvh * G + row) * D + d0) = o;
+    return;
+  }
+  const size_t at = ((size_t)(seq * p.Hkv + kvh) * p.num_parts + part) * G + row;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) p.part_o[at * D + d0 + j] = acc[j] * inv;
+  if ((threadIdx.x & 15) == 0) {
+    p.part_m[at] = M;
+    p.part_l[at] = L;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- prompts
+// A workgroup takes a tile of 32 NW flattened rows (token and head of the kv head's group), a wave 32 of them, and
+// 64 keys at a time, which all waves have widened into LDS, while the next ones' codes are on their way to
+// registers.  Products 32 x 32 x 16; a lane column is a query row.
+__device__ __forceinline__ float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// row r of a 32-key product holds this key: then the 8 accumulator registers that a lane half hands on as
+// weights are the keys of one 8-token group
+__device__ __forceinline__ int row_key(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
+
+constexpr int kKeys = 64;
+
+template <int NW>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p) {
+  constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
+  __shared__ __attribute__((aligned(16))) bf16 lds[2][2][kKeys * D];    // [buffer][K | V]
+  const int flat = gridDim.x - 1 - blockIdx.x;     // the map rises by work: longest tiles first
+  const int tile = flat / p.Hkv, kvh = flat - tile * p.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int seq = __builtin_amdgcn_readfirstlane(p.tile_seq[tile]);
+  const int q0 = p.q_start[seq], q_len = p.q_start[seq + 1] - q0;
+  const int ctx = p.seq_lens[seq] - q_len, keys = keys_of(p, seq);
+  const int G = p.G, BS = p.BS, row0 = p.tile_row[tile];
+  const int R = row0 + 32 * w + r, pos = R / G, hig = R - pos * G;
+  const bool valid = pos < q_len;
+  const int limit = valid ? min(ctx + pos, keys - 1) : -1;
+
+  // Q^T: lane (r, h) holds dims 16 s + 8 h .. + 7 of its row
+  bf16x8 qf[8];
+  {
+    const int t = valid ? pos : 0;
+    const bool prep = p.qkv != nullptr;
+    const bf16* src = (prep ? p.qkv + (size_t)(q0 + t) * p.qkv_stride : p.q + (size_t)(q0 + t) * p.Hq * D) +
+                      (kvh * G + hig) * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(src + 16 * s);
+    if (prep) {
+      float x[8][8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] = bf2f(qf[s][j]);
+      if (p.q_w != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) ss += x[s][j] * x[s][j];
+        const float inv = rsqrtf(half_sum(ss) * (1.f / D) + p.eps);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const bf16x8 nw = *reinterpret_cast<const bf16x8*>(p.q_w + 16 * s + 8 * h);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[s][j] = x[s][j] * inv * bf2f(nw[j]);
+        }
+      }
+      const int64_t at = p.positions[q0 + t];
+      const float* cs = p.cos_sin + (size_t)(at < 0 ? 0 : at < p.max_pos ? at : p.max_pos - 1) * D + 8 * h;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float c = cs[16 * s + j], sn = cs[64 + 16 * s + j];
+          qf[s][j] = f2bf(x[s][j] * c - x[s + 4][j] * sn);
+          qf[s + 4][j] = f2bf(x[s + 4][j] * c + x[s][j] * sn);
+        }
+    }
+  }
+
+  const int last_pos = min(q_len - 1, (row0 + ROWS - 1) / G);
+  const int ntiles = last_pos < 0 ? 0 : (min(ctx + last_pos, keys - 1) + kKeys) / kKeys;
+  const int w_first = (row0 + 32 * w) / G;
+  const bool active = w_first < q_len;
+  const int w_limit = ctx + min(q_len - 1, (row0 + 32 * w + 31) / G), w_min = min(ctx + w_first, keys - 1);
+
+  // pieces: 512 of K and 512 of V to a tile; a wave's lie in one 32-key chunk
+  const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
+  const int chunk = (w * PW * 64) >> 8;
+  u32x4 kc[PW], vc[PW];
+  float ks = 1.f, vs = 1.f;
+  // a chunk's page, or -1 where it lies behind the keys or outside the cache
+  auto page_of = [&](int c) -> int {
+    if (32 * c >= keys) return -1;
+    const int b = bt[32 * c / BS];
+    return (uint32_t)b < (uint32_t)p.num_blocks ? b : -1;
+  };
+  auto fetch = [&](int t) {
+    const int c = 2 * t + chunk, b = __builtin_amdgcn_readfirstlane(page_of(c));
+    if (b < 0) {
+#pragma unroll
+      for (int i = 0; i < PW; ++i) kc[i] = vc[i] = u32x4{0, 0, 0, 0};
+      return;
+    }
+    const int64_t at = ((int64_t)b * p.Hkv + kvh) * BS * D + (int64_t)(32 * c % BS) * D;
+    ks = p.k_scale[(size_t)b * p.Hkv + kvh];
+    vs = p.v_scale[(size_t)b * p.Hkv + kvh];
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int pc = (tid * PW + i) & 255;
+      kc[i] = *reinterpret_cast<const u32x4*>(p.k_cache + at + pc * 16);
+      vc[i] = *reinterpret_cast<const u32x4*>(p.v_cache + at + pc * 16);
+    }
+    if (32 * c + 32 > keys) {      // values behind the last key may be no numbers: zeros
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {
+        const int mine = keys - 32 * c - 8 * (((tid * PW + i) & 255) >> 6);
+        const uint32_t lo = mine >= 4 ? ~0u : mine <= 0 ? 0u : (1u << (8 * mine)) - 1;
+        const uint32_t hi = mine >= 8 ? ~0u : mine <= 4 ? 0u : (1u << (8 * (mine - 4))) - 1;
+        vc[i] = u32x4{vc[i][0] & lo, vc[i][1] & hi, vc[i][2] & lo, vc[i][3] & hi};
+      }
+    }
+  };
+  // K image: token rows of 256 bytes, 16-byte column c of row k at c ^ (k & 15); V image: the groups as they are
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int pc = (tid * PW + i) & 255;       // K: [half 2][dims / 32 4][row 16][2]
+      const int col = 4 * ((pc >> 5) & 3) + 2 * (pc & 1), r16 = (pc >> 1) & 15;
+      const int key = 32 * chunk + 8 * (r16 >> 2) + 4 * (pc >> 7) + (r16 & 3);
+      bf16* kl = lds[buf][0] + key * D;
+      *reinterpret_cast<bf16x8*>(kl + (col ^ (key & 15)) * 8) = codes_wide(kc[i][0], kc[i][1], ks);
+      *reinterpret_cast<bf16x8*>(kl + ((col + 1) ^ (key & 15)) * 8) = codes_wide(kc[i][2], kc[i][3], ks);
+      bf16* vl = lds[buf][1] + (chunk * 256 + pc) * 16;
+      *reinterpret_cast<bf16x8*>(vl) = codes_wide(vc[i][0], vc[i][1], vs);
+      *reinterpret_cast<bf16x8*>(vl + 8) = codes_wide(vc[i][2], vc[i][3], vs);
+    }
+  };
+
+  f32x16 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  float m = -1e30f, l = 0.f;
+  if (ntiles > 0) {
+    fetch(0);
+    store(0);
+  }
+  __syncthreads();
+  for (int t = 0; t < ntiles; ++t) {
+    const bool more = t + 1 < ntiles;
+    if (more) fetch(t + 1);
+    const int key0 = t * kKeys;
+    if (active && key0 <= w_limit) {
+      const bf16* kl = lds[t & 1][0];
+      const bf16* vl = lds[t & 1][1];
+      f32x16 s[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[k][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int key = 32 * k + row_key(r);
+          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kl + key * D + ((2 * i + h) ^ (key & 15)) * 8);
+          s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i], s[k], 0, 0, 0);
+        }
+      const bool lost0 = page_of(2 * t) < 0, lost1 = page_of(2 * t + 1) < 0;    // uniform
+      float top = -INFINITY;
+      if (key0 + kKeys - 1 > w_min || lost0 || lost1) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || (k ? lost1 : lost0)) s[k][j] = -INFINITY;
+            top = fmaxf(top, s[k][j]);
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, s[k][j]);
+      }
+      const float mn = fmaxf(m, half_max(top) * p.scale_log2), a = __builtin_amdgcn_exp2f(m - mn);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          s[k][j] = __builtin_amdgcn_exp2f(fmaf(s[k][j], p.scale_log2, -mn));
+          sum += s[k][j];
+        }
+      l = l * a + half_sum(sum);
+      if (__any(mn != m)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[i][j] *= a;
+      }
+      m = mn;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          bf16x8 pb;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pb[j] = f2bf(s[k][8 * s2 + j]);
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            const bf16x8 vf = *reinterpret_cast<const bf16x8*>(vl + ((4 * k + 2 * s2 + h) * D + 32 * dt + r) * 8);
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[dt], 0, 0, 0);
+          }
+        }
+    }
+    if (more) store((t + 1) & 1);
+    __syncthreads();
+  }
+  // dims 32 dt + 8 i + 4 h .. + 3 of a row to a lane
+  if (!valid) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  bf16* to = p.out + ((size_t)(q0 + pos) * p.Hq + kvh * G + hig) * D + 4 * h;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bf16x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = f2bf(o[dt][4 * i + j] * inv);
+      *reinterpret_cast<bf16x4*>(to + 32 * dt + 8 * i) = x;
+    }
+}
+
+}  // namespace
+
+void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
+  if (num_seqs == 0) return;
+  const size_t smem = (size_t)(4 * p.G * (D + 4) + 8 * p.G) * sizeof(float);
+  scaled_decode_kernel<<<dim3(num_seqs, p.Hkv, p.num_parts), 256, smem, s>>>(p);
+  if (p.num_parts > 1) scaled_merge_kernel<<<dim3(num_seqs, p.Hkv), 256, 0, s>>>(p);
+}
+
+void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, hipStream_t s) {
+  if (num_tiles == 0) return;
+  if (tile_rows == 256) scaled_prefill_kernel<8><<<num_tiles * p.Hkv, 512, 0, s>>>(p);
+  else scaled_prefill_kernel<4><<<num_tiles * p.Hkv, 256, 0, s>>>(p);
+}
+
+}  // namespace akap

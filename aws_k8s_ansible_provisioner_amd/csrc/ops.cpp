@@ -326,6 +326,226 @@ void paged_attention_decode_fused(Tensor out, Tensor qkv, Tensor k_cache, Tensor
   akap::launch_paged_attn_decode(p, B, cur_stream());
 }
 
+// ---- the scaled 8-bit cache (scaled_cache.hip, scaled_attention.hip) ----
+// Shapes of a layer's cache: K [NB, Hkv, BS, 128], V [NB, Hkv, BS/8, 128, 8] bytes, scales [2, NB, Hkv] fp32.
+static void check_scaled(const Tensor& k_cache, const Tensor& v_cache, const Tensor& scales) {
+  CHECK_GPU(k_cache); CHECK_CONTIG(k_cache); CHECK_CONTIG(v_cache); CHECK_CONTIG(scales);
+  TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
+              "scaled cache: uint8 K and V (e4m3 codes)");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(3) == 128, "scaled cache: K [NB, Hkv, BS, 128]");
+  TORCH_CHECK(k_cache.size(2) > 0 && k_cache.size(2) % 32 == 0, "scaled cache: block size must be a multiple of 32");
+  TORCH_CHECK(v_cache.dim() == 5 && v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) &&
+                  v_cache.size(2) * 8 == k_cache.size(2) && v_cache.size(3) == 128 && v_cache.size(4) == 8,
+              "scaled cache: V [NB, Hkv, BS/8, 128, 8]");
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.dim() == 3 && scales.size(0) == 2 &&
+                  scales.size(1) == k_cache.size(0) && scales.size(2) == k_cache.size(1),
+              "scaled cache: scales fp32 [2, NB, Hkv]");
+  TORCH_CHECK(k_cache.size(0) < (1LL << 31) && (uintptr_t)k_cache.data_ptr() % 16 == 0 &&
+                  (uintptr_t)v_cache.data_ptr() % 16 == 0,
+              "scaled cache: caches must lie on 16 bytes");
+}
+
+static void check_same_device(const Tensor& a, std::initializer_list<const Tensor*> others) {
+  for (const Tensor* t : others)
+    TORCH_CHECK(t->device() == a.device(), "all tensors must be on one device");
+}
+
+// rows of the projection: bf16, on 16 bytes, wide enough for all heads
+static void check_rows(const Tensor& qkv, int64_t heads) {
+  CHECK_GPU(qkv); CHECK_BF16(qkv);
+  TORCH_CHECK(qkv.dim() == 2 && qkv.stride(1) == 1 && qkv.size(1) >= heads * 128,
+              "qkv: rows of (Hq + 2 Hkv) * 128 or more, unit last stride");
+  TORCH_CHECK(qkv.stride(0) % 8 == 0 && (uintptr_t)qkv.data_ptr() % 16 == 0, "qkv rows must be 16-byte aligned");
+}
+static void check_norm_weight(const Tensor& qkv, const std::optional<Tensor>& w) {
+  if (!w) return;
+  CHECK_BF16(*w);
+  TORCH_CHECK(w->is_contiguous() && w->numel() == 128 && (uintptr_t)w->data_ptr() % 16 == 0,
+              "norm weights: contiguous bf16 [128] on 16 bytes");
+  check_same_device(qkv, {&*w});
+}
+static void check_angles(const Tensor& qkv, const Tensor& positions, const Tensor& cos_sin, int64_t rows) {
+  TORCH_CHECK(positions.scalar_type() == at::kLong && positions.is_contiguous() && positions.numel() >= rows,
+              "positions: int64, one per row");
+  TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.dim() == 2 &&
+                  cos_sin.size(1) == 128 && cos_sin.size(0) > 0 && (uintptr_t)cos_sin.data_ptr() % 16 == 0,
+              "cos_sin: contiguous fp32 [max_pos, 128]");
+  check_same_device(qkv, {&positions, &cos_sin});
+}
+
+void scaled_cache_append(Tensor qkv, Tensor q_out, Tensor k_cache, Tensor v_cache, Tensor scales,
+                         Tensor positions, Tensor slots, Tensor cos_sin, std::optional<Tensor> q_w,
+                         std::optional<Tensor> k_w, int64_t Hq, int64_t Hkv, double eps, bool apply_rope,
+                         int64_t singles, int64_t q_rows) {
+  check_scaled(k_cache, v_cache, scales);
+  TORCH_CHECK(Hq >= 0 && Hkv == k_cache.size(1), "scaled_cache_append: the cache has other kv heads");
+  check_rows(qkv, Hq + 2 * Hkv);
+  const int64_t T = qkv.size(0);
+  TORCH_CHECK(T < (1LL << 31) && singles >= 0 && singles <= T && q_rows >= -1 && q_rows <= T,
+              "scaled_cache_append: num_decode / q_rows out of range");
+  if (q_rows < 0) q_rows = T;
+  check_angles(qkv, positions, cos_sin, T);
+  check_norm_weight(qkv, q_w);
+  check_norm_weight(qkv, k_w);
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() >= T,
+              "slots: int64, one per row");
+  check_same_device(qkv, {&q_out, &k_cache, &v_cache, &scales, &slots});
+  if (q_rows > 0) {
+    CHECK_BF16(q_out); CHECK_CONTIG(q_out);
+    TORCH_CHECK(q_out.numel() >= q_rows * Hq * 128 && (uintptr_t)q_out.data_ptr() % 16 == 0,
+                "q_out: contiguous bf16 rows of Hq * 128, one for each row whose q is written");
+  }
+  akap::ScaledAppend p{};
+  p.qkv = (const __bf16*)qkv.data_ptr();
+  p.qkv_stride = qkv.stride(0);
+  p.q_out = (__bf16*)q_out.data_ptr();
+  p.k_cache = k_cache.data_ptr<uint8_t>();
+  p.v_cache = v_cache.data_ptr<uint8_t>();
+  p.k_scale = scales.data_ptr<float>();
+  p.v_scale = p.k_scale + scales.size(1) * scales.size(2);
+  p.positions = positions.data_ptr<int64_t>();
+  p.slots = slots.data_ptr<int64_t>();
+  p.cos_sin = cos_sin.data_ptr<float>();
+  p.q_w = q_w ? (const __bf16*)q_w->data_ptr() : nullptr;
+  p.k_w = k_w ? (const __bf16*)k_w->data_ptr() : nullptr;
+  p.T = T;
+  p.q_rows = q_rows;
+  p.singles = singles;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.BS = k_cache.size(2);
+  p.num_blocks = k_cache.size(0);
+  p.max_pos = cos_sin.size(0);
+  p.eps = (float)eps;
+  p.rope = apply_rope ? 1 : 0;
+  const c10::DeviceGuard g(qkv.device());
+  akap::launch_scaled_append(p, cur_stream());
+}
+
+static akap::ScaledAttn scaled_params(const Tensor& out, const Tensor& k_cache, const Tensor& v_cache,
+                                      const Tensor& scales, const Tensor& block_tables, const Tensor& seq_lens,
+                                      int64_t G, double scale) {
+  check_scaled(k_cache, v_cache, scales);
+  CHECK_GPU(out); CHECK_BF16(out); CHECK_CONTIG(out);
+  TORCH_CHECK(out.dim() == 3 && out.size(2) == 128 && (uintptr_t)out.data_ptr() % 16 == 0, "out: [T, Hq, 128]");
+  TORCH_CHECK(G > 0 && out.size(1) == k_cache.size(1) * G, "Hq must equal Hkv * G");
+  TORCH_CHECK(block_tables.scalar_type() == at::kInt && block_tables.dim() == 2 && block_tables.size(1) > 0 &&
+                  block_tables.stride(1) == 1,
+              "block_tables: int32 [B, blocks], rows contiguous");
+  TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.is_contiguous() &&
+                  block_tables.size(0) >= seq_lens.numel(),
+              "seq_lens: contiguous int32, a block table for each");
+  TORCH_CHECK(scale > 0 && scale < 1e30, "the score scale must be positive");
+  check_same_device(out, {&k_cache, &v_cache, &scales, &block_tables, &seq_lens});
+  akap::ScaledAttn p{};
+  p.k_cache = k_cache.data_ptr<uint8_t>();
+  p.v_cache = v_cache.data_ptr<uint8_t>();
+  p.k_scale = scales.data_ptr<float>();
+  p.v_scale = p.k_scale + scales.size(1) * scales.size(2);
+  p.out = (__bf16*)out.data_ptr();
+  p.block_tables = block_tables.data_ptr<int>();
+  p.bt_stride = block_tables.stride(0);
+  p.bt_cols = block_tables.size(1);
+  p.seq_lens = seq_lens.data_ptr<int>();
+  p.Hq = out.size(1);
+  p.Hkv = k_cache.size(1);
+  p.G = G;
+  p.BS = k_cache.size(2);
+  p.num_blocks = k_cache.size(0);
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  return p;
+}
+
+static void check_query(const Tensor& out, const Tensor& q) {
+  CHECK_BF16(q); CHECK_CONTIG(q);
+  TORCH_CHECK(q.sizes() == out.sizes() && (uintptr_t)q.data_ptr() % 16 == 0, "q: bf16, shaped like out");
+  check_same_device(out, {&q});
+}
+
+// partitions of a decode step and what holds their rows
+static void set_parts(akap::ScaledAttn& p, const Tensor& out, int64_t B, int64_t num_parts, int64_t part_size,
+                      const Tensor& part_m, const Tensor& part_l, const Tensor& part_o,
+                      const std::optional<Tensor>& tickets) {
+  TORCH_CHECK(num_parts > 0 && num_parts < 65536 && part_size > 0 && part_size % 128 == 0 &&
+                  part_size <= akap::kDecodeMaxPart,
+              "part_size must be a multiple of 128, at most ", akap::kDecodeMaxPart);
+  TORCH_CHECK(num_parts == 1 || part_size % p.BS == 0, "partitions must hold whole blocks");
+  TORCH_CHECK(B < (1LL << 31) && p.Hkv < 65536, "too many rows");
+  p.num_parts = num_parts;
+  p.part_size = part_size;
+  if (num_parts == 1) return;
+  for (const Tensor* t : {&part_m, &part_l, &part_o})
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous(), "workspace: contiguous fp32");
+  const int64_t rows = B * p.Hkv * num_parts * p.G;
+  TORCH_CHECK(part_m.numel() >= rows && part_l.numel() >= rows && part_o.numel() >= rows * 128,
+              "workspace too small for ", num_parts, " partitions of ", B, " rows");
+  check_same_device(out, {&part_m, &part_l, &part_o});
+  p.part_m = part_m.data_ptr<float>();
+  p.part_l = part_l.data_ptr<float>();
+  p.part_o = part_o.data_ptr<float>();
+}
+
+void scaled_attention_decode(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor scales,
+                             Tensor block_tables, Tensor seq_lens, std::optional<Tensor> q_start, Tensor part_m,
+                             Tensor part_l, Tensor part_o, int64_t num_parts, int64_t part_size, int64_t G,
+                             double scale, std::optional<Tensor> tickets) {
+  auto p = scaled_params(out, k_cache, v_cache, scales, block_tables, seq_lens, G, scale);
+  check_query(out, q);
+  TORCH_CHECK(G <= 16, "decode kernel supports up to 16 q heads per kv head");
+  const int64_t B = seq_lens.numel();
+  if (q_start) {
+    TORCH_CHECK(q_start->scalar_type() == at::kInt && q_start->is_contiguous() && q_start->numel() >= B,
+                "q_start: int32, a row for each sequence");
+    check_same_device(out, {&*q_start});
+    p.q_start = q_start->data_ptr<int>();
+  } else {
+    TORCH_CHECK(out.size(0) >= B, "out: a row for each sequence");
+  }
+  p.q = (const __bf16*)q.data_ptr();
+  set_parts(p, out, B, num_parts, part_size, part_m, part_l, part_o, tickets);
+  const c10::DeviceGuard g(out.device());
+  akap::launch_scaled_decode(p, B, cur_stream());
+}
+
+void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional<Tensor> qkv, Tensor k_cache,
+                              Tensor v_cache, Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start,
+                              Tensor tile_seq, Tensor tile_row, std::optional<Tensor> positions,
+                              std::optional<Tensor> cos_sin, std::optional<Tensor> q_w, int64_t G, double scale,
+                              double eps, int64_t tile_rows) {
+  auto p = scaled_params(out, k_cache, v_cache, scales, block_tables, seq_lens, G, scale);
+  TORCH_CHECK(tile_rows == 128 || tile_rows == 256, "tile_rows must be 128 or 256");
+  const int64_t B = seq_lens.numel();
+  for (const Tensor* t : {&q_start, &tile_seq, &tile_row})
+    TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), "q_start / tile maps must be contiguous int32");
+  TORCH_CHECK(q_start.numel() >= B + 1 && tile_row.numel() >= tile_seq.numel(), "q_start / tile maps too short");
+  check_same_device(out, {&q_start, &tile_seq, &tile_row});
+  TORCH_CHECK(tile_seq.numel() * p.Hkv < (1LL << 31) && out.size(0) * G < (1LL << 31), "too many rows");
+  if (qkv) {
+    TORCH_CHECK(positions && cos_sin, "rows of the projection need positions and cos_sin");
+    check_rows(*qkv, out.size(1) + 2 * k_cache.size(1));
+    TORCH_CHECK(qkv->size(0) == out.size(0), "qkv / out token counts differ");
+    check_angles(*qkv, *positions, *cos_sin, out.size(0));
+    check_norm_weight(*qkv, q_w);
+    check_same_device(out, {&*qkv});
+    p.qkv = (const __bf16*)qkv->data_ptr();
+    p.qkv_stride = qkv->stride(0);
+    p.positions = positions->data_ptr<int64_t>();
+    p.cos_sin = cos_sin->data_ptr<float>();
+    p.max_pos = cos_sin->size(0);
+    p.q_w = q_w ? (const __bf16*)q_w->data_ptr() : nullptr;
+    p.eps = (float)eps;
+  } else {
+    TORCH_CHECK(q, "scaled_attention_prefill: q or qkv");
+    check_query(out, *q);
+    p.q = (const __bf16*)q->data_ptr();
+  }
+  p.q_start = q_start.data_ptr<int>();
+  p.tile_seq = tile_seq.data_ptr<int>();
+  p.tile_row = tile_row.data_ptr<int>();
+  const c10::DeviceGuard g(out.device());
+  akap::launch_scaled_prefill(p, tile_seq.numel(), (int)tile_rows, cur_stream());
+}
+
 void l2_prefetch(std::vector<Tensor> ts, Tensor sink) {
   TORCH_CHECK(ts.size() <= 8, "at most 8 tensors");
   akap::PrefetchList L{};
@@ -1340,6 +1560,18 @@ TORCH_LIBRARY(akap, m) {
       "Tensor(f!) part_o, int num_parts, int part_size, int G, float scale, float eps, "
       "Tensor(g!)? v_tail=None, Tensor? tail_slot=None, Tensor(h!)? tickets=None) -> ()");
   m.def(
+      "scaled_cache_append(Tensor qkv, Tensor(a!) q_out, Tensor(b!) k_cache, Tensor(c!) v_cache, "
+      "Tensor(d!) scales, Tensor positions, Tensor slots, Tensor cos_sin, Tensor? q_w, Tensor? k_w, int Hq, "
+      "int Hkv, float eps, bool apply_rope, int singles=0, int q_rows=-1) -> ()");
+  m.def(
+      "scaled_attention_decode(Tensor(a!) out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor scales, "
+      "Tensor block_tables, Tensor seq_lens, Tensor? q_start, Tensor(b!) part_m, Tensor(c!) part_l, "
+      "Tensor(d!) part_o, int num_parts, int part_size, int G, float scale, Tensor(e!)? tickets=None) -> ()");
+  m.def(
+      "scaled_attention_prefill(Tensor(a!) out, Tensor? q, Tensor? qkv, Tensor k_cache, Tensor v_cache, "
+      "Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start, Tensor tile_seq, Tensor tile_row, "
+      "Tensor? positions, Tensor? cos_sin, Tensor? q_w, int G, float scale, float eps, int tile_rows=128) -> ()");
+  m.def(
       "sample(Tensor logits, Tensor temperature, Tensor top_k, Tensor top_p, Tensor seeds, "
       "Tensor steps, Tensor(a!) out_tokens, Tensor(b!) out_logprobs, "
       "bool greedy_logprobs, Tensor(c!) ws, Tensor(d!) tickets, bool filtered=True) -> ()");
@@ -1435,6 +1667,9 @@ TORCH_LIBRARY_IMPL(akap, CUDA, m) {
   m.impl("paged_attention_prefill_qprep", &paged_attention_prefill_qprep);
   m.impl("paged_attention_decode", &paged_attention_decode);
   m.impl("paged_attention_decode_fused", &paged_attention_decode_fused);
+  m.impl("scaled_cache_append", &scaled_cache_append);
+  m.impl("scaled_attention_decode", &scaled_attention_decode);
+  m.impl("scaled_attention_prefill", &scaled_attention_prefill);
   m.impl("sample", &sample);
   m.impl("apply_penalties", &apply_penalties);
   m.impl("argmax", &argmax);

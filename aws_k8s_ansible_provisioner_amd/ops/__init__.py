@@ -295,6 +295,168 @@ def _decode_workspace(max_seqs: int, num_kv_heads: int, gqa_group: int, num_part
     return pm, pl, po
 
 
+# ----------------------------------------------------------------------------- scaled 8-bit cache
+# A layer's cache in 8 bits with a scale for each block of tokens and kv head: K and V as uint8 in the
+# layouts above, holding e4m3 codes, and `scales` fp32 [2, NB, Hkv], the power of two that a block's codes
+# of K (scales[0]) and of V (scales[1]) are multiplied with.  The least scale that holds all of a block's
+# entries up to 448 times it, from 2^-100 to 2^100: set anew by the append that writes a block's first
+# token, kept or raised by others, which round the block's other codes anew where they raise it.
+# Infinities are kept as the largest number, NaN as 0 and neither counts towards the scale.
+def scaled_cache_scales(num_layers: int, num_blocks: int, num_kv_heads: int, device=None) -> torch.Tensor:
+    """Scales [num_layers, 2, num_blocks, num_kv_heads] of caches that hold nothing yet."""
+    return torch.full((num_layers, 2, num_blocks, num_kv_heads), 2.0 ** -ref.SCALE_EXP,
+                      dtype=torch.float32, device=device)
+
+
+def _check_scaled(k_cache, v_cache, scales) -> None:
+    """The checks of csrc/ops.cpp check_scaled for CPU tensors."""
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+        raise RuntimeError("scaled cache: uint8 K and V (e4m3 codes)")
+    if k_cache.dim() != 4 or k_cache.shape[2] % 32 or k_cache.shape[3] % 32:
+        raise RuntimeError("scaled cache: K [NB, Hkv, BS, D], block size a multiple of 32")
+    NB, H, BS, D = k_cache.shape
+    if tuple(v_cache.shape) != (NB, H, BS // 8, D, 8):
+        raise RuntimeError("scaled cache: V [NB, Hkv, BS/8, D, 8]")
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (2, NB, H):
+        raise RuntimeError("scaled cache: scales fp32 [2, NB, Hkv]")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and scales.is_contiguous()):
+        raise RuntimeError("scaled cache: caches and scales must be contiguous")
+
+
+def _check_scaled_attention(out, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group, scale):
+    _check_scaled(k_cache, v_cache, scales)
+    if gqa_group <= 0 or out.dim() != 3 or out.shape[1] != k_cache.shape[1] * gqa_group:
+        raise RuntimeError("Hq must equal Hkv * G")
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise RuntimeError("block_tables / seq_lens must be int32")
+    if block_tables.dim() != 2 or block_tables.shape[0] < seq_lens.numel():
+        raise RuntimeError("block_tables: int32 [B, blocks], one for each sequence")
+    if not 0 < scale < 1e30:
+        raise RuntimeError("the score scale must be positive")
+
+
+def check_scaled_slots(slots, block_size: int) -> None:
+    """Raise unless a call's rows of one block stand together, in rising slots (what the append kernel
+    takes for granted: a wave owns a block's entries of the call)."""
+    s = [int(x) for x in slots.tolist()]
+    seen = set()
+    for i, x in enumerate(s):
+        if x < 0:
+            continue
+        follows = i > 0 and s[i - 1] == x - 1 and x % block_size
+        if not follows:
+            if x // block_size in seen:
+                raise RuntimeError(f"scaled_cache_append: row {i} (slot {x}) is apart from its block's others")
+            seen.add(x // block_size)
+
+
+def scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin, q_w, k_w,
+                        num_q_heads: int, num_kv_heads: int, eps: float, apply_rope: bool = True,
+                        decode: bool = False, num_decode: int = 0, q_rows: int = -1):
+    """qk_norm_rope_cache for a scaled cache: per-head norms (q_w, k_w; None: none) and rotation of the
+    projection's rows [q heads | k heads | v heads], q to q_out (of the first q_rows rows, -1: of all), k and
+    v as codes into their slots.  All in fp32 up to the one rounding of each result.  A negative slot, or one
+    outside the cache, has no entry.  The rows of a block must stand together in rising slots
+    (check_scaled_slots).  decode: every row is a single token of its sequence (num_decode: the leading ones
+    are); that only divides the work."""
+    if _native(qkv):
+        if DEBUG_CHECKS:
+            check_scaled_slots(slots[:qkv.shape[0]], k_cache.shape[2])
+        torch.ops.akap.scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin,
+                                           q_w, k_w, num_q_heads, num_kv_heads, eps, apply_rope,
+                                           qkv.shape[0] if decode else num_decode, q_rows)
+        return q_out
+    _check_scaled(k_cache, v_cache, scales)
+    T, D = qkv.shape[0], k_cache.shape[3]
+    if num_kv_heads != k_cache.shape[1]:
+        raise RuntimeError("scaled_cache_append: the cache has other kv heads")
+    if qkv.dim() != 2 or qkv.shape[1] < (num_q_heads + 2 * num_kv_heads) * D:
+        raise RuntimeError("qkv: rows of (Hq + 2 Hkv) * D or more")
+    if not (0 <= num_decode <= T and -1 <= q_rows <= T):
+        raise RuntimeError("scaled_cache_append: num_decode / q_rows out of range")
+    if positions.dtype != torch.int64 or slots.dtype != torch.int64 or min(positions.numel(), slots.numel()) < T:
+        raise RuntimeError("positions / slots: int64, one per row")
+    check_scaled_slots(slots[:T], k_cache.shape[2])
+    ref.scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin, q_w, k_w,
+                            num_q_heads, num_kv_heads, eps, apply_rope, q_rows)
+    return q_out
+
+
+def scaled_attention_decode(out, q, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group: int,
+                            scale: float, workspace=None, num_parts: int = 1, part_size: int = 512,
+                            q_start=None):
+    """paged_attention_decode over a scaled cache: one row per sequence (row q_start[b], or b) over its
+    seq_lens[b] keys.  num_parts * part_size must hold the longest sequence's keys, part_size whole blocks
+    where there are several.  A key of a block table entry outside the cache is left out; a row that sees no
+    key is zero."""
+    if _native(q):
+        if workspace is None:
+            workspace = _decode_workspace(seq_lens.numel(), k_cache.shape[1], gqa_group, num_parts, q.device)
+        pm, pl, po = workspace
+        torch.ops.akap.scaled_attention_decode(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start,
+                                               pm, pl, po, num_parts, part_size, gqa_group, scale,
+                                               getattr(workspace, "tickets", None))
+        return out
+    _check_scaled_attention(out, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group, scale)
+    _check_parts(k_cache, num_parts, part_size)
+    B = seq_lens.numel()
+    at = torch.arange(B) if q_start is None else q_start[:B].long()
+    rows = torch.empty(B, *out.shape[1:], dtype=out.dtype)
+    ref.scaled_attention(rows, q[at], k_cache, v_cache, scales, block_tables, seq_lens,
+                         torch.arange(B + 1), scale)
+    out[at] = rows
+    return out
+
+
+def _check_parts(k_cache, num_parts: int, part_size: int) -> None:
+    if num_parts <= 0 or part_size <= 0 or part_size % 128 or part_size > DECODE_MAX_PART:
+        raise RuntimeError(f"part_size must be a multiple of 128, at most {DECODE_MAX_PART}")
+    if num_parts > 1 and part_size % k_cache.shape[2]:
+        raise RuntimeError("partitions must hold whole blocks")
+
+
+def scaled_attention_decode_fused(out, qkv, k_cache, v_cache, scales, block_tables, seq_lens, positions,
+                                  slots, cos_sin, q_w, k_w, gqa_group: int, scale: float, eps: float,
+                                  workspace=None, num_parts: int = 1, part_size: int = 512):
+    """A decode step over a scaled cache from the projection's rows: scaled_cache_append of one new token per
+    sequence, then scaled_attention_decode of its normed and rotated q (as bf16).  out [B, Hq, D]."""
+    B, Hq, D = out.shape
+    Hkv = k_cache.shape[1]
+    q = torch.empty_like(out)
+    scaled_cache_append(qkv[:B], q, k_cache, v_cache, scales, positions, slots, cos_sin, q_w, k_w, Hq, Hkv,
+                        eps, True, decode=True)
+    return scaled_attention_decode(out, q, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group, scale,
+                                   workspace, num_parts, part_size)
+
+
+def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start, tile_seq,
+                             tile_row, gqa_group: int, scale: float, tile_rows: int = 128, qprep=None):
+    """paged_attention_prefill over a scaled cache: causal attention of each sequence's rows q_start[b] ..
+    q_start[b + 1] - 1, its last tokens, over its seq_lens[b] keys; the tile map as there (tile_rows 128 or
+    256; sequences that no tile names are left as they are).
+    qprep = (qkv, positions, cos_sin, q_w, eps): the kernel takes its q rows from the projection's, normed and
+    rotated by their positions, rounded to bf16 (q is not read then and may be None)."""
+    if _native(out):
+        qkv, positions, cos_sin, q_w, eps = qprep if qprep is not None else (None, None, None, None, 0.0)
+        torch.ops.akap.scaled_attention_prefill(out, None if qprep is not None else q, qkv, k_cache, v_cache,
+                                                scales, block_tables, seq_lens, q_start, tile_seq, tile_row,
+                                                positions, cos_sin, q_w, gqa_group, scale, eps, tile_rows)
+        return out
+    _check_scaled_attention(out, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group, scale)
+    if tile_rows not in (64, 128, 256):
+        raise RuntimeError("tile_rows must be 128 or 256")
+    if qprep is not None:
+        qkv, positions, cos_sin, q_w, eps = qprep
+        T, Hq, D = out.shape
+        x = qkv[:T, :Hq * D].float().view(T, Hq, D)
+        if q_w is not None:
+            x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * q_w.float()
+        q = ref.apply_rope(x, positions[:T].clamp(0, cos_sin.shape[0] - 1), cos_sin).to(torch.bfloat16)
+    ref.scaled_attention(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start, scale,
+                         keep=None if tile_seq is None else set(tile_seq.tolist()))
+    return out
+
+
 # ----------------------------------------------------------------------------- GEMM
 _GEMM_MODE = os.environ.get("AKAP_GEMM", "torch")  # torch (hipBLASLt) | auto | hip
 GEMM_MAX_M = int(os.environ.get("AKAP_GEMM_MAX_M", "512"))

@@ -185,6 +185,105 @@ def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, q_start, scale)
     return out
 
 
+# ---------------------------------------------------------------------------- scaled 8-bit cache
+SCALE_EXP = 100  # scales lie between 2^-100 and 2^100
+
+
+def cache_scale(most: torch.Tensor) -> torch.Tensor:
+    """The least power of two (2^-100 .. 2^100) with `most` <= 448 times it."""
+    m, e = torch.frexp(most.float())     # most = m 2^e, 0.5 <= m < 1; 448 = 0.875 * 2^9
+    e = torch.where(most > 0, e - 9 + (m > 0.875).to(e.dtype), torch.full_like(e, -SCALE_EXP))
+    return torch.ldexp(torch.ones_like(m), e.clamp(-SCALE_EXP, SCALE_EXP))
+
+
+def to_codes(x: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """x / scale as e4m3 codes (uint8): to nearest even, infinities the largest number, NaN 0."""
+    y = torch.nan_to_num(x.float() / scale, nan=0.0, posinf=FP8_MAX, neginf=-FP8_MAX)
+    return y.clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+def scaled_tokens(k_cache, v_cache, scales, pages):
+    """Codes and scales of `pages` in token order: two [len(pages), BS, Hkv, D] uint8 and two
+    [len(pages), Hkv]."""
+    NB, H, BS, D = k_cache.shape
+    k = k_blocks_view(k_cache)[pages].permute(0, 2, 3, 5, 1, 4, 6)
+    k = k.reshape(len(pages), BS // 32, 32, H, D)[:, :, K_CHUNK_POS].reshape(len(pages), BS, H, D)
+    v = v_cache[pages].permute(0, 2, 4, 1, 3).reshape(len(pages), BS, H, D)
+    return k, v, scales[0, pages], scales[1, pages]
+
+
+def scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin, q_w, k_w,
+                        Hq, Hkv, eps, apply_rope_flag=True, q_rows=-1):
+    T = qkv.shape[0]
+    NB, _, BS, D = k_cache.shape
+    x = qkv[:, :(Hq + 2 * Hkv) * D].float().view(T, Hq + 2 * Hkv, D)
+
+    def prepared(y, w):
+        if w is not None:
+            y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        if apply_rope_flag:
+            y = apply_rope(y, positions[:T].clamp(0, cos_sin.shape[0] - 1), cos_sin)
+        return y
+
+    n = T if q_rows < 0 else q_rows
+    if n and Hq:
+        q_out.view(-1, Hq * D)[:n].copy_(prepared(x[:, :Hq], q_w)[:n].reshape(n, -1).to(q_out.dtype))
+    kv = (prepared(x[:, Hq:Hq + Hkv], k_w), x[:, Hq + Hkv:])
+    slots = slots[:T].long()
+    rows = torch.nonzero((slots >= 0) & (slots < NB * BS)).flatten()
+    if not len(rows):
+        return
+    at, off = slots[rows] // BS, slots[rows] % BS
+    pages, row = torch.unique(at, return_inverse=True)
+    fresh = torch.zeros(len(pages), dtype=torch.bool)
+    fresh[row[off == 0]] = True
+    k, v, *_ = scaled_tokens(k_cache, v_cache, scales, pages)
+    for j, (codes, new) in enumerate(((k, kv[0][rows]), (v, kv[1][rows]))):
+        mag = torch.where(torch.isfinite(new), new.abs(), torch.zeros(())).amax(-1)   # [rows, Hkv]
+        need = torch.zeros(len(pages), Hkv).scatter_reduce_(0, row[:, None].expand_as(mag), mag, "amax")
+        need, old = cache_scale(need), scales[j, pages]
+        scale = torch.where(fresh[:, None], need, torch.maximum(old, need))
+        ratio = torch.where(fresh[:, None], torch.ones(()), old / scale)[:, None, :, None]
+        grown = to_codes(codes.view(torch.float8_e4m3fn).float() * ratio, torch.ones(()))
+        codes = torch.where(ratio < 1, grown, codes)
+        codes[row, off] = to_codes(new, scale[row][..., None])
+        scales[j, pages] = scale
+        if j:
+            v_cache[pages] = codes.view(-1, BS // 8, 8, Hkv, D).permute(0, 3, 1, 4, 2)
+        else:
+            order = [K_CHUNK_POS.index(i) for i in range(32)]
+            c = codes.view(-1, BS // 32, 32, Hkv, D)[:, :, order].view(-1, BS // 32, 2, 16, Hkv, D // 32, 32)
+            k_blocks_view(k_cache)[pages] = c.permute(0, 4, 1, 2, 5, 3, 6)
+
+
+def scaled_attention(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start, scale,
+                     keep=None):
+    """Causal attention of each sequence's last rows over the scaled cache, written to out's rows of
+    sequences with at least one (`keep`: those of these sequences alone).  Keys behind the table or of a
+    page outside the cache are left out; a row that sees none is zero."""
+    NB, Hkv, BS, D = k_cache.shape
+    G = q.shape[1] // Hkv
+    for b in range(seq_lens.numel()):
+        q0, n = int(q_start[b]), int(q_start[b + 1]) - int(q_start[b])
+        if n <= 0 or (keep is not None and b not in keep):
+            continue
+        kv = int(seq_lens[b])
+        pages = block_tables[b, :max(0, -(-kv // BS))].long()
+        good = (pages >= 0) & (pages < NB)
+        k, v, ks, vs = scaled_tokens(k_cache, v_cache, scales, pages.clamp(0, NB - 1))
+        k, v = ((c.view(torch.float8_e4m3fn).float() * s[:, None, :, None]).reshape(-1, Hkv, 1, D)
+                .expand(-1, -1, G, -1).reshape(-1, Hkv * G, D) for c, s in ((k, ks), (v, vs)))
+        key = torch.arange(k.shape[0])
+        seen = (key[None] <= torch.arange(kv - n, kv)[:, None]) & good.repeat_interleave(BS)[None]
+        # (what stands behind the sequence's end, or in no page, may be no number)
+        dead = ~((key < kv) & good.repeat_interleave(BS))
+        k, v = (t.masked_fill(dead[:, None, None], 0.0) for t in (k, v))
+        s = torch.einsum("qhd,khd->hqk", q[q0:q0 + n].float(), k) * scale
+        s = s.masked_fill(~seen[None], float("-inf"))
+        p = torch.softmax(s, dim=-1).masked_fill(~seen.any(-1)[None, :, None], 0.0)
+        out[q0:q0 + n] = torch.einsum("hqk,khd->qhd", p, v).to(out.dtype)
+
+
 def sample(logits, temperature, top_k, top_p, seeds, steps, greedy_logprobs=False):
     """Reference sampler: greedy for T<=0; else top-k, then top-p (on the top-k
     renormalised distribution), then a draw.  Draws use torch's RNG seeded per row,
