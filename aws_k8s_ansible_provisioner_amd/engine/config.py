@@ -3,6 +3,7 @@ llm-d style manifests and the reference's smoke test keep working)."""
 from __future__ import annotations
 
 import dataclasses
+import math
 from typing import Optional
 
 
@@ -27,7 +28,9 @@ class EngineConfig:
     weights_path: Optional[str] = None
     chat_template: Optional[str] = None
     kv_role: str = "both"                     # "both" | "prefill" | "decode" (P/D)
-    kv_cache_dtype: str = "auto"              # "auto" (model dtype, bf16) | "fp8" (e4m3fn)
+    # "auto" (model dtype, bf16) | "fp8" (e4m3fn, scale 1) | "fp8_scaled" (e4m3fn with a power-of-two
+    # scale for each block and kv head: any range of keys and values; one process, no P/D roles)
+    kv_cache_dtype: str = "auto"
     init_std: float = 0.02                    # random-init weight scale
     shard_init: str = "per_rank"              # "per_rank" | "full" (identical logical weights for any TP)
     mixed_batching: bool = True               # decodes + prefill chunks in one step
@@ -49,8 +52,18 @@ class EngineConfig:
             raise ValueError(f"block_size must be a multiple of 32, got {self.block_size}")
         if self.dtype not in ("bfloat16", "float32"):
             raise ValueError(f"dtype must be bfloat16 or float32, got {self.dtype}")
-        if self.kv_cache_dtype not in ("auto", "bf16", "bfloat16", "fp8", "fp8_e4m3"):
-            raise ValueError(f"kv_cache_dtype must be auto or fp8, got {self.kv_cache_dtype}")
+        if self.kv_cache_dtype not in ("auto", "bf16", "bfloat16", "fp8", "fp8_e4m3", "fp8_scaled"):
+            raise ValueError("kv_cache_dtype must be auto, fp8 or fp8_scaled, got "
+                             f"{self.kv_cache_dtype}")
+        if self.scaled_kv and self.kv_role != "both":
+            raise ValueError("kv_cache_dtype fp8_scaled: P/D roles move codes without their scales")
+        if self.scaled_kv and math.lcm(self.block_size, 128) > 8192:
+            raise ValueError(f"kv_cache_dtype fp8_scaled: no decode partition of at most 8192 tokens holds "
+                             f"whole blocks of {self.block_size}")
+
+    @property
+    def scaled_kv(self) -> bool:
+        return self.kv_cache_dtype == "fp8_scaled"
 
     def resolved_device(self) -> str:
         if self.device != "auto":

@@ -95,14 +95,14 @@ class ModelRunner:
         # 301.6 us, Llama-3-8B 32 x 512: 149.2 vs 154.5, 4 x 4096: 566.3 vs 578.8, q prep in
         # the kernel), the 128-row tile on chunks whose every prompt has <= 1024 rows (Qwen3
         # 32 x 512: 83.8 vs 87.9 us) -- profiles/r6_prefill_tile_order.md.  The 256-row kernel
-        # needs a bf16 KV cache.
-        bf16_kv = dev == "cuda" and not ecfg.kv_cache_dtype.startswith("fp8")
+        # needs a bf16 KV cache, or a scaled one.
+        bf16_kv = dev == "cuda" and (not ecfg.kv_cache_dtype.startswith("fp8") or ecfg.scaled_kv)
         self.tile_rows = 256 if bf16_kv else (128 if dev == "cuda" else 64)
         self.tile_rows_short = 128 if bf16_kv else 0
         if dev == "cuda" and os.environ.get("AKAP_PREFILL_TILE_ROWS") in ("128", "256"):
             self.tile_rows = int(os.environ["AKAP_PREFILL_TILE_ROWS"])  # A/B knob
             self.tile_rows_short = 0
-            if self.tile_rows == 256 and ecfg.kv_cache_dtype.startswith("fp8"):
+            if self.tile_rows == 256 and not bf16_kv:
                 self.tile_rows = 128  # the 256-row kernel needs a bf16 KV cache
         if tile_plan is not None:
             self.G, self.tile_rows, self.tile_rows_short = tile_plan()
@@ -125,7 +125,12 @@ class ModelRunner:
         gib = sum(t.numel() * t.element_size() for t in self.kv_segs) / 2**30
         self.log(f"[runner] KV cache: {self.num_blocks} blocks x {self.bs} tokens "
                  f"({gib:.1f} GiB in {len(self.kv_segs)} allocation(s), "
-                 f"{'fp8 e4m3' if self.kv_dtype == torch.uint8 else 'bf16'})")
+                 f"{ecfg.kv_cache_dtype if self.kv_dtype == torch.uint8 else 'bf16'})")
+        # scaled cache: each layer's scales [2, blocks, kv heads] beside its codes
+        self.kv_scales: Optional[list] = None
+        if ecfg.scaled_kv:
+            self.kv_scales = list(ops.scaled_cache_scales(mcfg.num_layers, self.num_blocks, self.model.hkv,
+                                                          self.device).unbind(0))
         # V tail (see AttnParams.v_tail): one slot per live sequence (2x max_num_seqs, as P/D
         # activations can briefly exceed it; a sequence without a slot uses the plain path)
         self.v_tails: Optional[list] = None
@@ -209,6 +214,8 @@ class ModelRunner:
             per_block = self.model.kv_block_bytes(self.bs, self.ecfg.kv_cache_dtype)
         else:
             per_block = self.mcfg.num_layers * 2 * self.model.hkv * self.bs * self.model.D * elem
+            if self.ecfg.scaled_kv:
+                per_block += self.mcfg.num_layers * 2 * self.model.hkv * 4
         if not self.is_gpu:
             return max(64, min(4096, (self.max_seqs * self.ecfg.max_model_len) // self.bs + 8))
         torch.cuda.synchronize()
@@ -449,7 +456,8 @@ class ModelRunner:
         batch = AttnBatch(True, pos, slots, bt, sl, qs, ts, tr, parts, ps,
                           self.workspace, tile_rows=info.get("tile_rows") or self.tile_rows,
                           num_decode=nd,
-                          v_tails=self.v_tails, tail_slot=v["tail_slot"])
+                          v_tails=self.v_tails, tail_slot=v["tail_slot"],
+                          kv_scales=self.kv_scales)
         if self._ep_moe:
             moe_mod.ep_overflow_reset(self.device)
         h = self.model.forward(ids, batch, self.k_caches, self.v_caches)
@@ -535,8 +543,10 @@ class ModelRunner:
             parts = min(math.ceil(2048 / wgs), max(1, math.ceil(max_len / 256)))
         # a partition is at most ops.DECODE_MAX_PART tokens (the kernel holds one block id
         # per 128-token wave step in a VGPR lane: 64 steps)
-        parts = max(parts, math.ceil(max_len / ops.DECODE_MAX_PART))
-        ps = math.ceil(math.ceil(max_len / parts) / 128) * 128
+        # (of a scaled cache also whole blocks: a block's scale is one work item's)
+        unit = math.lcm(128, self.bs) if self.kv_scales is not None else 128
+        parts = max(parts, math.ceil(max_len / (ops.DECODE_MAX_PART // unit * unit)))
+        ps = math.ceil(math.ceil(max_len / parts) / unit) * unit
         parts = math.ceil(max_len / ps)
         return parts, ps
 
@@ -559,7 +569,7 @@ class ModelRunner:
         batch = AttnBatch(False, dd["positions"][:n], dd["slots"][:n], self.dd_bt[:n],
                           dd["seq_lens"][:n], self.d["q_start"][:n + 1], None, None,
                           parts, ps, self.workspace, v_tails=self.v_tails,
-                          tail_slot=dd["tail_slot"][:n])
+                          tail_slot=dd["tail_slot"][:n], kv_scales=self.kv_scales)
         h = self.model.forward(dd["input_ids"][:n], batch, self.k_caches, self.v_caches)
         # sampler reads bf16 logits directly (no [n, V] fp32 cast pass)
         logits = self.model.compute_logits(h)

@@ -55,6 +55,8 @@ class AttnBatch:
     # per-token (= per decode row) tail slot; None = the plain V cache write path
     v_tails: Optional[list] = None
     tail_slot: Optional[torch.Tensor] = None
+    # scaled 8-bit cache: per-layer scales [2, blocks, kv heads]; None = the other caches
+    kv_scales: Optional[list] = None
 
 
 @dataclasses.dataclass
@@ -311,7 +313,8 @@ class DecoderLM:
         """Layer-range segments [Ls, 2, NB, Hkv*BS*D] (K block = [Hkv,BS,D], V block =
         [Hkv,BS/8,D,8]) of at most `max_segment_bytes` each (AKAP_KV_SEGMENT_GIB, default 32),
         zero-filled so never-written slots read as finite zeros.  kv_dtype "fp8": uint8
-        storage of OCP e4m3fn values (half the bytes of bf16).  Each segment is its own
+        storage of OCP e4m3fn values (half the bytes of bf16), with "fp8_scaled" codes whose scales the
+        runner keeps beside them.  Each segment is its own
         allocation, exported by hipIpc on its own (P/D pull).
 
         On the GPU every allocation's size is kept hipIpc-safe (`ipc_safe_alloc_bytes`): the
@@ -355,6 +358,45 @@ class DecoderLM:
     def embed_tokens(self, ids: torch.Tensor) -> torch.Tensor:
         x = ops.embedding(ids, self.embed, vocab_start=self.vocab_start, vocab_end=self.vocab_end)
         return comm.tp_all_reduce(x)
+
+    def _decode_fused(self, out, qkv, batch: AttnBatch, kc, vc, lw, li: int):
+        """A decode step's attention straight from the projection rows."""
+        G = self.hq // self.hkv
+        if batch.kv_scales is not None:
+            ops.scaled_attention_decode_fused(
+                out, qkv, kc, vc, batch.kv_scales[li], batch.block_tables, batch.seq_lens,
+                batch.positions, batch.slots, self.cos_sin, lw.q_norm, lw.k_norm, G, self.scale,
+                self.cfg.rms_eps, workspace=batch.workspace, num_parts=batch.num_parts,
+                part_size=batch.part_size)
+            return
+        ops.paged_attention_decode_fused(
+            out, qkv, kc, vc, batch.block_tables, batch.seq_lens, batch.positions, batch.slots,
+            self.cos_sin, lw.q_norm, lw.k_norm, G, self.scale, self.cfg.rms_eps,
+            workspace=batch.workspace, num_parts=batch.num_parts, part_size=batch.part_size,
+            v_tail=batch.v_tails[li] if batch.v_tails is not None else None,
+            tail_slot=batch.tail_slot)
+
+    def _scaled_attention(self, out, qkv, batch: AttnBatch, kc, vc, lw, li: int):
+        """A step over a scaled cache in separate launches: append, then the single rows, then the
+        prompts (on the GPU those prepare their own query rows from the projection's)."""
+        G, nd, sc = self.hq // self.hkv, batch.num_decode, batch.kv_scales[li]
+        prompts = batch.is_prefill
+        q = torch.empty_like(out)
+        qp = prompts and PREFILL_QPREP and qkv.is_cuda
+        ops.scaled_cache_append(qkv, q, kc, vc, sc, batch.positions, batch.slots, self.cos_sin,
+                                lw.q_norm, lw.k_norm, self.hq, self.hkv, self.cfg.rms_eps,
+                                decode=not prompts, num_decode=nd if prompts else 0,
+                                q_rows=nd if qp else -1)
+        n = nd if prompts else batch.seq_lens.numel()
+        if n:
+            ops.scaled_attention_decode(out[:n], q[:n], kc, vc, sc, batch.block_tables[:n],
+                                        batch.seq_lens[:n], G, self.scale, workspace=batch.workspace,
+                                        num_parts=batch.num_parts, part_size=batch.part_size)
+        if prompts:
+            ops.scaled_attention_prefill(
+                out, q, kc, vc, sc, batch.block_tables, batch.seq_lens, batch.q_start, batch.tile_seq,
+                batch.tile_row, G, self.scale, tile_rows=batch.tile_rows,
+                qprep=(qkv, batch.positions, self.cos_sin, lw.q_norm, self.cfg.rms_eps) if qp else None)
 
     def _attention(self, q, batch: AttnBatch, kc, vc, out, vt=None, qprep=None):
         if batch.is_prefill:
@@ -409,12 +451,9 @@ class DecoderLM:
             vt = batch.v_tails[li] if batch.v_tails is not None else None
             if not batch.is_prefill and FUSED_DECODE:
                 # q/k-norm + RoPE + KV-cache write fused into the decode attention kernel
-                ops.paged_attention_decode_fused(
-                    attn, qkv, k_caches[li], v_caches[li], batch.block_tables, batch.seq_lens,
-                    batch.positions, batch.slots, self.cos_sin, lw.q_norm, lw.k_norm,
-                    self.hq // self.hkv, self.scale, eps, workspace=batch.workspace,
-                    num_parts=batch.num_parts, part_size=batch.part_size, v_tail=vt,
-                    tail_slot=batch.tail_slot)
+                self._decode_fused(attn, qkv, batch, k_caches[li], v_caches[li], lw, li)
+            elif batch.kv_scales is not None:
+                self._scaled_attention(attn, qkv, batch, k_caches[li], v_caches[li], lw, li)
             else:
                 q = torch.empty_like(attn)
                 # prefill on the GPU: the attention kernel norms + rotates its own q rows from
@@ -486,13 +525,7 @@ class DecoderLM:
             attn = torch.empty(T, self.hq, self.D, dtype=self.dtype, device=self.device)
             if PREFETCH_WEIGHTS:  # A/B knob: warm the layer's remaining weights in MALL
                 ops.l2_prefetch([lw.w_o, lw.w_gate_up, lw.w_down, nxt])
-            ops.paged_attention_decode_fused(
-                attn, qkv, k_caches[li], v_caches[li], batch.block_tables, batch.seq_lens,
-                batch.positions, batch.slots, self.cos_sin, lw.q_norm, lw.k_norm,
-                self.hq // self.hkv, self.scale, eps, workspace=batch.workspace,
-                num_parts=batch.num_parts, part_size=batch.part_size,
-                v_tail=batch.v_tails[li] if batch.v_tails is not None else None,
-                tail_slot=batch.tail_slot)
+            self._decode_fused(attn, qkv, batch, k_caches[li], v_caches[li], lw, li)
             a2 = torch.empty_like(residual)
             if tp > 1:
                 part = ops.dgemm(attn.view(T, self.hq * self.D), lw.w_o, eps=eps, **c_o)

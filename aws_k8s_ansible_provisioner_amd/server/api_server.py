@@ -634,9 +634,10 @@ def make_parser() -> argparse.ArgumentParser:
     ap.add_argument("--kv-store-port", type=int,
                     default=int(os.environ.get("AKAP_KV_STORE_PORT", "29710")),
                     help="--pd-bootstrap http, prefill role: TCPStore port of the pair channels")
-    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8", "fp8_e4m3"],
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8", "fp8_e4m3", "fp8_scaled"],
                     help="fp8: OCP e4m3 KV cache (half the bytes; decode attention streams "
-                         "half as much)")
+                         "half as much); fp8_scaled: with a scale for each block and kv head, "
+                         "for keys and values of any range")
     ap.add_argument("--otlp-traces-endpoint", default=None,
                     help="OTLP/HTTP collector (e.g. http://otel-collector:4318); also read "
                          "from OTEL_EXPORTER_OTLP_TRACES_ENDPOINT")

@@ -55,9 +55,9 @@ def parse():
                     help="KV cache blocks per engine (0: sized from free memory)")
     ap.add_argument("--temperature", type=float, default=0.0)
     ap.add_argument("--enforce-eager", action="store_true")
-    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"],
-                    help="fp8 = e4m3 KV cache (NOT the headline config: bf16 KV like the "
-                         "reference's vLLM default)")
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8", "fp8_scaled"],
+                    help="fp8 = e4m3 KV cache, fp8_scaled = with block scales (NOT the headline "
+                         "config: bf16 KV like the reference's vLLM default)")
     ap.add_argument("--device", default="auto")
     ap.add_argument("--tp", type=int, default=1,
                     help="tensor-parallel degree: with --tp WORLD_SIZE the whole job is ONE "
@@ -499,7 +499,8 @@ def main() -> int:
                 "max_num_seqs": a.max_num_seqs,
                 "sampling": "greedy" if a.temperature <= 0 else f"T={a.temperature}",
                 "hipgraph_decode": not a.enforce_eager,
-                "kv_cache_dtype": "bf16" if a.kv_cache_dtype == "auto" else "fp8_e4m3",
+                "kv_cache_dtype": {"auto": "bf16", "fp8": "fp8_e4m3"}.get(a.kv_cache_dtype,
+                                                                    a.kv_cache_dtype),
                 "mixed_batching": not a.no_mixed_batching,
             },
         }

@@ -215,3 +215,32 @@ def test_rows_of_a_block_apart_are_refused():
     for slots in ([5, 5], [6, 5], [5, 7], [5, -1, 6]):
         with pytest.raises(RuntimeError):
             ops.check_scaled_slots(torch.tensor(slots), 32)
+
+
+# ------------------------------------------------------------------------------------------------ engine
+def test_engine_on_a_scaled_cache():
+    """--kv-cache-dtype fp8_scaled: greedy tokens near the argmax of the dense reference, also where keys are far
+    beyond the largest code."""
+    from test_engine_cpu import _engine, _near_argmax
+    from aws_k8s_ansible_provisioner_amd.engine.config import SamplingParams
+
+    eng = _engine("tiny-qwen3", kv_cache_dtype="fp8_scaled")
+    assert eng.runner.kv.dtype == torch.uint8 and len(eng.runner.kv_scales) == eng.runner.mcfg.num_layers
+    prompts = [list(range(5, 45)), [7, 8, 9] * 14]
+    outs = eng.generate(None, SamplingParams(max_tokens=8, temperature=0, ignore_eos=True), prompt_ids=prompts)
+    for p, o in zip(prompts, outs):
+        _near_argmax(eng, p, o.output_ids, tol=0.5)
+    for s in eng.runner.kv_scales:
+        assert bool((s > 2.0 ** -100).any()) and bool((torch.frexp(s)[0] == 0.5).all())
+
+
+def test_engine_refuses_roles_and_blocks():
+    from aws_k8s_ansible_provisioner_amd.engine.config import EngineConfig
+
+    for kw in (dict(kv_role="prefill"), dict(kv_role="decode"), dict(block_size=8192 + 32),
+               dict(block_size=96 * 32 + 32)):
+        with pytest.raises(ValueError):
+            EngineConfig(kv_cache_dtype="fp8_scaled", **kw)
+    EngineConfig(kv_cache_dtype="fp8_scaled", block_size=96)
+    with pytest.raises(ValueError):
+        EngineConfig(kv_cache_dtype="fp8_other")

@@ -400,3 +400,35 @@ def test_offsets_past_32_bits():
     ops.scaled_attention_decode(one, q[69:].contiguous(), k, v, s, table.to(DEV), n, 1, 0.1)
     close(one, *orc.attention(q[69:], entries, here, [70], [0, 1], 0.1))
     assert not k[:pages - 3].any() and not v[:pages - 3].any()
+
+
+# ------------------------------------------------------------------------------------------------ engine
+@pytest.mark.parametrize("model", ["tiny-qwen3", "tiny-llama"])
+@pytest.mark.parametrize("block", [32, 96])
+def test_engine_on_a_scaled_cache(model, block):
+    """--kv-cache-dtype fp8_scaled end to end: prompts, captured decode steps, mixed steps."""
+    from test_engine_gpu import _check_teacher_forced, _engine
+    from aws_k8s_ansible_provisioner_amd.engine.config import SamplingParams
+
+    eng = _engine(model, kv_cache_dtype="fp8_scaled", block_size=block)
+    assert eng.runner.kv.dtype == torch.uint8 and eng.runner.graphs
+    prompts = [list(range(3, 80)), [17] * 33 + [5, 6, 7]]
+    outs = eng.generate(None, SamplingParams(max_tokens=10, temperature=0, ignore_eos=True), prompt_ids=prompts)
+    for p, o in zip(prompts, outs):
+        assert len(o.output_ids) == 10
+        _check_teacher_forced(eng, p, o.output_ids, tol=0.6)
+    sp = SamplingParams(max_tokens=12, temperature=0, ignore_eos=True)
+    eng.add_request("a", None, sp, prompt_ids=list(range(5, 90)))
+    got, mixed = {}, False
+    for step in range(100):
+        if step == 3:
+            eng.add_request("b", None, sp, prompt_ids=[9, 8, 7] * 30)
+        for o in eng.step():
+            if o.finished:
+                got[o.req_id] = o.output_ids
+        mixed |= eng.last_step_mixed
+        if len(got) == 2:
+            break
+    assert mixed
+    _check_teacher_forced(eng, list(range(5, 90)), got["a"], tol=0.6)
+    _check_teacher_forced(eng, [9, 8, 7] * 30, got["b"], tol=0.6)
