@@ -119,10 +119,10 @@ void launch_scaled_append(const ScaledAppend& p, hipStream_t s);
 
 struct ScaledAttn {
   const __bf16* q;           // [T, Hq, D]
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
-  const float* k_scale;
-  const float* v_scale;
+  uint8_t* k_cache;          // (written by the fused decode alone)
+  uint8_t* v_cache;
+  float* k_scale;
+  float* v_scale;
   __bf16* out;               // [T, Hq, D]
   const int* block_tables;   // [B, bt_cols], rows bt_stride apart
   int64_t bt_stride;
@@ -138,13 +138,16 @@ struct ScaledAttn {
   int* tickets;              // as in AttnParams
   const int* tile_seq;       // prompts: each tile's sequence and first flattened row
   const int* tile_row;
-  // rows as the projection gave them (prompts, fused decode): normed and rotated by the kernel
+  // rows as the projection gave them (prompts, fused decode): normed and rotated by the kernel; fused decode: the
+  // new key and value appended to slots[b]
   const __bf16* qkv;
   int64_t qkv_stride;
   const int64_t* positions;
+  const int64_t* slots;
   const float* cos_sin;
   int64_t max_pos;
   const __bf16* q_w;
+  const __bf16* k_w;
   float eps;
 };
 void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s);

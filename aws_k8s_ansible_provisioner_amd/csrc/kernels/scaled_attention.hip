@@ -5,6 +5,8 @@
 //
 // A key is seen if it lies inside the sequence's length, the block table and a page of the cache (a table entry
 // outside the cache: its keys are left out).  A row that sees none is zero.
+#include <algorithm>
+
 #include "scaled_cache.h"
 #include "kernels.h"
 
@@ -22,26 +24,35 @@ __device__ __forceinline__ int keys_of(const ScaledAttn& p, int seq) {
 }
 
 // ------------------------------------------------------------------------------------------------- decode
-// grid (sequences, kv heads, partitions), four waves that take a partition's 32-token chunks in turn; the rows of
+// grid (sequences, kv heads, partitions), four waves that take a partition's 32-token chunks in turn; the columns of
 // the 16 x 16 x 32 products are the kv head's query heads.  A chunk is 8 loads of 16 bytes to a lane: of K the dims
 // 64 p + 16 g .. + 15 of a token (its k-steps 2 p and 2 p + 1 contract over the first and second 8, q in the same
-// order), of V two dims of an 8-token group.
+// order), of V two dims of an 8-token group.  The next chunk's K is asked for when this one's scores are formed, its
+// V when this one's is used up: a whole chunk on the way in the registers of one.
 struct Chunk {
   u32x4 k[2][2];   // [16-token tile][p]
   u32x4 v[4];      // dims 32 n + 2 r and + 1 of group g
 };
+constexpr int kStream = 2;     // buffer instructions: read once a step, not kept in the caches
 
-__device__ __forceinline__ void chunk_load(Chunk& c, const ScaledAttn& p, int64_t page, int in_page) {
+// the 32-token chunk of a cache that begins at byte `at`; 0 and nothing read where there is none
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rsrc(const uint8_t* cache, int64_t at, bool some) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(cache + at), (short)0, some ? 32 * D : 0, 0x00020000);
+}
+__device__ __forceinline__ void load_k(Chunk& c, __amdgpu_buffer_rsrc_t rs) {
   const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-  const uint8_t* kb = p.k_cache + page + (size_t)in_page * D + (g >> 1) * 512 + r * 32 + (g & 1) * 16;
-  const uint8_t* vb = p.v_cache + page + (size_t)(in_page / 8 + g) * D * 8 + r * 16;
+  const int at = (g >> 1) * 512 + r * 32 + (g & 1) * 16;
 #pragma unroll
   for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      c.k[tt][i] = ld_nt(reinterpret_cast<const u32x4*>(kb + tt * 2048 + i * 1024));
+      c.k[tt][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + tt * 2048 + i * 1024, 0, kStream));
+}
+__device__ __forceinline__ void load_v(Chunk& c, __amdgpu_buffer_rsrc_t rs) {
+  const int lane = threadIdx.x & 63, at = (lane >> 4) * D * 8 + (lane & 15) * 16;
 #pragma unroll
-  for (int n = 0; n < 4; ++n) c.v[n] = ld_nt(reinterpret_cast<const u32x4*>(vb + n * 256));
+  for (int n = 0; n < 4; ++n)
+    c.v[n] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, at + n * 256, 0, kStream));
 }
 
 struct Row {
@@ -49,11 +60,8 @@ struct Row {
   float m, l;      // running maximum (log2), this lane's part of the sum
 };
 
-// END: the chunk holds keys from `end` on that are not seen (and may hold any codes)
-template <bool END>
-__device__ __forceinline__ void chunk_take(Row& st, const bf16x8 (&q)[4], Chunk& c, float kscale, float vscale,
-                                           int left) {
-  const int g = (threadIdx.x & 63) >> 4;
+// scores of tokens 8 g + 0..7 of the chunk
+__device__ __forceinline__ void chunk_scores(float (&x)[8], const bf16x8 (&q)[4], const Chunk& c, float kscale) {
   f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -62,13 +70,21 @@ __device__ __forceinline__ void chunk_take(Row& st, const bf16x8 (&q)[4], Chunk&
       s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_wide(c.k[tt][i][0], c.k[tt][i][1], 1.f), q[2 * i], s[tt], 0, 0, 0);
       s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_wide(c.k[tt][i][2], c.k[tt][i][3], 1.f), q[2 * i + 1], s[tt], 0, 0, 0);
     }
-  float x[8], top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {      // token 8 g + i of the chunk
-    x[i] = s[i >> 2][i & 3] * kscale;
-    if (END && 8 * g + i >= left) x[i] = -INFINITY;
-    top = fmaxf(top, x[i]);
+  for (int i = 0; i < 8; ++i) x[i] = s[i >> 2][i & 3] * kscale;
+}
+
+// left: the chunk's keys that are seen; the others may hold any codes.  (One body with small branches: a second one
+// for whole chunks took the kernel from 126 registers to 202, from four waves a SIMD to two.)
+__device__ __forceinline__ void chunk_rows(Row& st, float (&x)[8], Chunk& c, float vscale, int left) {
+  const int g = (threadIdx.x & 63) >> 4;
+  if (left < 32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 8 * g + i < left ? x[i] : -INFINITY;
   }
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
   top = fmaxf(top, __shfl_xor(top, 16, 64));
   top = fmaxf(top, __shfl_xor(top, 32, 64));
   const float m = fmaxf(st.m, top), a = __builtin_amdgcn_exp2f(st.m - m);
@@ -82,7 +98,7 @@ __device__ __forceinline__ void chunk_take(Row& st, const bf16x8 (&q)[4], Chunk&
     w[i] = f2bf(e);
   }
   st.l = st.l * a + sum;
-  if (END) {                         // what lies behind the end may be no number: zeros
+  if (left < 32) {                   // values that are not seen may be no numbers: zeros
     const int mine = left - 8 * g;
     const uint32_t lo = mine >= 4 ? ~0u : mine <= 0 ? 0u : (1u << (8 * mine)) - 1;
     const uint32_t hi = mine >= 8 ? ~0u : mine <= 4 ? 0u : (1u << (8 * (mine - 4))) - 1;
@@ -99,73 +115,248 @@ __device__ __forceinline__ void chunk_take(Row& st, const bf16x8 (&q)[4], Chunk&
     }
 }
 
-// The partitions of a (sequence, kv head): 16 threads to a row, 8 dims to a thread.
-__device__ __forceinline__ void merge(const ScaledAttn& p, int seq, int kvh, int nparts, int q_tok) {
-  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
-  if (row >= p.G) return;
-  const size_t base = (size_t)(seq * p.Hkv + kvh) * p.num_parts * p.G + row;
+// Partial rows: those of a launch that merges its own go past the XCDs' caches.
+constexpr int kPast = 16;
+template <bool SHARED>
+__device__ __forceinline__ float part_load(const float* at) {
+  return SHARED ? __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *at;
+}
+
+// The partitions of a (sequence, kv head) into its rows: 16 threads to a row, 8 dims to a thread, 16 / (G rounded
+// up to a power of two) groups of threads that take every so many-th partition, eight of them requested together.
+// lds: 16 rows of D + 4.
+template <bool SHARED>
+__device__ __forceinline__ void merge(const ScaledAttn& p, int seq, int kvh, int nparts, int q_tok, float* lds) {
+  constexpr int U = 8;
+  const int G = p.G, wide = G <= 1 ? 1 : 1 << (32 - __builtin_clz(G - 1));
+  const int at16 = threadIdx.x >> 4, row = at16 & (wide - 1), first = at16 / wide, groups = 16 / wide;
+  const int d0 = (threadIdx.x & 15) * 8;
+  const int64_t base = (int64_t)(seq * p.Hkv + kvh) * p.num_parts * G;
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(p.part_o + base * D), (short)0, SHARED ? p.num_parts * G * D * 4 : 0, 0x00020000);
   float M = -1e30f, L = 0.f, acc[8] = {};
-  for (int i = 0; i < nparts; ++i) M = fmaxf(M, p.part_m[base + (size_t)i * p.G]);
-  for (int i = 0; i < nparts; ++i) {
-    const size_t at = base + (size_t)i * p.G;
-    const float f = __builtin_amdgcn_exp2f(p.part_m[at] - M) * p.part_l[at];
-    L += f;
+  if (row < G) {
+    for (int i0 = first; i0 < nparts; i0 += U * groups) {
+      float m[U], l[U];
+      f32x4 o[U][2];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += f * p.part_o[at * D + d0 + j];
+      for (int u = 0; u < U; ++u) {
+        const int at = min(i0 + u * groups, nparts - 1) * G + row;
+        m[u] = part_load<SHARED>(p.part_m + base + at);
+        l[u] = part_load<SHARED>(p.part_l + base + at);
+        if constexpr (SHARED) {
+          const int b = (at * D + d0) * 4;
+          o[u][0] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, b, 0, kPast));
+          o[u][1] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, b + 16, 0, kPast));
+        } else {
+          const float* po = p.part_o + (base + at) * D + d0;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) o[u][k] = f32x4{po[4 * k], po[4 * k + 1], po[4 * k + 2], po[4 * k + 3]};
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) top = fmaxf(top, m[u]);     // (the last partition again changes nothing)
+      const float a = __builtin_amdgcn_exp2f(M - top);
+      M = top;
+      L *= a;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] *= a;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * groups >= nparts) break;
+        const float f = __builtin_amdgcn_exp2f(m[u] - M) * l[u];
+        L += f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += f * o[u][j >> 2][j & 3];
+      }
+    }
   }
+  if (groups > 1 && nparts > 1) {
+    float* mine = lds + at16 * (D + 4);
+    *reinterpret_cast<f32x4*>(mine + d0) = f32x4{acc[0], acc[1], acc[2], acc[3]};
+    *reinterpret_cast<f32x4*>(mine + d0 + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
+    if (d0 == 0) {
+      mine[D] = M;
+      mine[D + 1] = L;
+    }
+    __syncthreads();
+    if (first > 0) return;
+    for (int i = 1; i < groups; ++i) {
+      const float* other = lds + (i * wide + row) * (D + 4);
+      const float top = fmaxf(M, other[D]), a = __builtin_amdgcn_exp2f(M - top), b = __builtin_amdgcn_exp2f(other[D] - top);
+      M = top;
+      L = L * a + other[D + 1] * b;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = acc[j] * a + other[d0 + j] * b;
+    }
+  }
+  if (row >= G || first > 0) return;
   const float inv = L > 0.f ? 1.f / L : 0.f;
   bf16x8 o;
 #pragma unroll
   for (int j = 0; j < 8; ++j) o[j] = f2bf(acc[j] * inv);
-  *reinterpret_cast<bf16x8*>(p.out + ((size_t)q_tok * p.Hq + kvh * p.G + row) * D + d0) = o;
+  *reinterpret_cast<bf16x8*>(p.out + ((size_t)q_tok * p.Hq + kvh * G + row) * D + d0) = o;
 }
 
 __global__ __launch_bounds__(256) void scaled_merge_kernel(ScaledAttn p) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const int seq = blockIdx.x, keys = keys_of(p, seq);
-  merge(p, seq, blockIdx.y, min(p.num_parts, (keys + p.part_size - 1) / p.part_size), p.q_start ? p.q_start[seq] : seq);
+  merge<false>(p, seq, blockIdx.y, min(p.num_parts, (keys + p.part_size - 1) / p.part_size),
+               p.q_start ? p.q_start[seq] : seq, lds);
 }
 
-__global__ __launch_bounds__(256, 2) void scaled_decode_kernel(ScaledAttn p) {
+// The fused form's rows, 16 threads to a row and 8 dims to a thread: the kv head's G query heads, its key, its value.
+// Asked for ahead of the first chunk.
+struct NewRow {
+  bf16x8 x, w;
+  f32x4 c[2], s[2];
+};
+__device__ __forceinline__ void new_row_load(NewRow& n, const ScaledAttn& p, int seq, int kvh) {
+  const int G = p.G, row = min((int)threadIdx.x >> 4, G + 1), j = threadIdx.x & 15;
+  const int head = row < G ? kvh * G + row : row == G ? p.Hq + kvh : p.Hq + p.Hkv + kvh;
+  n.x = *reinterpret_cast<const bf16x8*>(p.qkv + (size_t)seq * p.qkv_stride + head * D + 8 * j);
+  const bf16* w = row < G ? p.q_w : row == G ? p.k_w : nullptr;
+  n.w = w != nullptr ? *reinterpret_cast<const bf16x8*>(w + 8 * j) : bf16x8{};
+  const int64_t pos = p.positions[seq];
+  const f32x4* cs = reinterpret_cast<const f32x4*>(
+      p.cos_sin + (size_t)(pos < 0 ? 0 : pos < p.max_pos ? pos : p.max_pos - 1) * D + 8 * (j & 7));
+  n.c[0] = cs[0];
+  n.c[1] = cs[1];
+  n.s[0] = cs[16];
+  n.s[1] = cs[17];
+}
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp_mov<0xB1>(v));
+  v = fmaxf(v, dpp_mov<0x4E>(v));
+  v = fmaxf(v, dpp_mov<0x141>(v));
+  return fmaxf(v, dpp_mov<0x140>(v));
+}
+// q to LDS; where the partition holds the row's last key, the new key and value into their page, whose scales (or
+// -1: no slot) go to LDS too.  As the append kernel does it, by 16 threads.
+__device__ __forceinline__ void new_row_put(NewRow& n, const ScaledAttn& p, int seq, int kvh, bool writes, bf16* q_s,
+                                            float* scale_s) {
+  const int G = p.G, row = threadIdx.x >> 4, j = threadIdx.x & 15;
+  if (row >= G + 2) return;
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = bf2f(n.x[e]);
+  if (row <= G) norm_rotate(x, (row < G ? p.q_w : p.k_w) != nullptr, n.w, true, n.c, n.s, j, p.eps);
+  if (row < G) {
+    bf16x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = f2bf(x[e]);
+    *reinterpret_cast<bf16x8*>(q_s + row * D + 8 * j) = o;
+    return;
+  }
+  if (!writes) return;
+  const bool value = row > G;
+  const int64_t slot = p.slots[seq];
+  if (slot < 0 || slot >= (int64_t)p.num_blocks * p.BS) {
+    if (j == 0) scale_s[value] = -1.f;
+    return;
+  }
+  const int64_t at = slot / p.BS * p.Hkv + kvh;
+  const int off = (int)(slot % p.BS);
+  uint8_t* codes = (value ? p.v_cache : p.k_cache) + at * p.BS * D;
+  float* scale = (value ? p.v_scale : p.k_scale) + at;
+  float most = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) most = fmaxf(most, scale_mag(x[e]));
+  const int exp = page_exp<16>(row16_max(most), scale, codes, off, p.BS);
+  const float inv = exp_scale(-exp);
+  const uint32_t lo = codes4(x[0], x[1], x[2], x[3], inv), hi = codes4(x[4], x[5], x[6], x[7], inv);
+  if (!value) {
+    *reinterpret_cast<u32x2*>(codes + k_swz_offset(off) + k_dim_offset(8 * j)) = u32x2{lo, hi};
+  } else {
+    uint8_t* to = codes + (size_t)(off >> 3) * D * 8 + 64 * j + (off & 7);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to[8 * e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+  }
+  if (j == 0) scale_s[value] = exp_scale(exp);
+}
+
+template <bool FUSED>
+__global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int seq = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
   const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = p.G, BS = p.BS;
-  const int first = part * p.part_size, keys = keys_of(p, seq), end = min(keys, first + p.part_size);
+  const int first = part * p.part_size, t0 = first + 32 * w, tok = t0 + 128 * lane;
+  // page and scales of the wave's chunk `lane` (the host bounds a partition to 64 chunks a wave); the table's entry
+  // is asked for beside the length
+  const int column = tok / BS;
+  int page = p.block_tables[(size_t)seq * p.bt_stride + min(column, p.bt_cols - 1)];
+  const int keys = keys_of(p, seq), end = min(keys, first + p.part_size);
   const int q_tok = p.q_start ? p.q_start[seq] : seq;
-  if (p.num_parts > 1 && first >= keys) return;     // (the merge leaves it out)
-  // page and scales of the wave's chunk `lane` (the host bounds a partition to 64 chunks a wave)
-  const int t0 = first + 32 * w, tok = t0 + 128 * lane;
-  int page = -1;
-  float ks = 0.f, vs = 0.f;
-  if (tok < end) {
-    page = p.block_tables[(size_t)seq * p.bt_stride + tok / BS];
-    if ((uint32_t)page >= (uint32_t)p.num_blocks) page = -1;
-    if (page >= 0) {
-      ks = p.k_scale[(size_t)page * p.Hkv + kvh] * p.scale_log2;
-      vs = p.v_scale[(size_t)page * p.Hkv + kvh];
-    }
+  const int nparts = min(p.num_parts, (keys + p.part_size - 1) / p.part_size);
+  if (p.num_parts > 1 && first >= keys) {      // (the merge leaves it out)
+    if (p.tickets != nullptr && part == 0) merge<true>(p, seq, kvh, 0, q_tok, lds);
+    return;
   }
+  NewRow fresh;
+  if constexpr (FUSED) new_row_load(fresh, p, seq, kvh);
+  if (tok >= end || (uint32_t)page >= (uint32_t)p.num_blocks) page = -1;
+  const int64_t sc = (int64_t)max(page, 0) * p.Hkv + kvh;
+  float ks = p.k_scale[sc] * p.scale_log2, vs = p.v_scale[sc];
+  const int in_page = (tok - column * BS) * D;
+  // chunk i of the wave: asked for without a branch, so that what each wait is for is known
+  auto page_of = [&](int i) { return i < 64 ? __builtin_amdgcn_readlane(page, i & 63) : -1; };
+  auto rsrc_of = [&](const uint8_t* cache, int i) {
+    const int blk = page_of(i);
+    return chunk_rsrc(cache, ((int64_t)max(blk, 0) * p.Hkv + kvh) * BS * D + (blk < 0 ? 0 : __builtin_amdgcn_readlane(in_page, i & 63)),
+                      blk >= 0);
+  };
+  Chunk c;
+  load_k(c, rsrc_of(p.k_cache, 0));
+  load_v(c, rsrc_of(p.v_cache, 0));
   bf16x8 q[4];
-  const bf16* qp = p.q + ((size_t)q_tok * p.Hq + kvh * G + min(r, G - 1)) * D + 16 * g;
+  if constexpr (FUSED) {
+    bf16* q_s = reinterpret_cast<bf16*>(lds);            // [G][D]
+    float* scale_s = lds + G * D / 2;                    // the new entries' scales
+    const bool writes = keys > 0 && part == nparts - 1;
+    new_row_put(fresh, p, seq, kvh, writes, q_s, scale_s);
+    if (writes) {
+      // what was written is read again by the chunks of its page: whole pages lie in a partition
+      __syncthreads();
+      const int last = (keys - 1) / BS;
+      if (column == last && scale_s[0] >= 0.f) {
+        ks = scale_s[0] * p.scale_log2;
+        vs = scale_s[1];
+      }
+      if (t0 < end && t0 / BS == last) {
+        load_k(c, rsrc_of(p.k_cache, 0));
+        load_v(c, rsrc_of(p.v_cache, 0));
+      }
+    } else {                                             // the first chunk stays on its way
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+    }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    q[i] = *reinterpret_cast<const bf16x8*>(qp + 64 * (i >> 1) + 8 * (i & 1));
-    if (r >= G) q[i] = bf16x8{};
+    for (int i = 0; i < 4; ++i)
+      q[i] = *reinterpret_cast<const bf16x8*>(q_s + min(r, G - 1) * D + 16 * g + 64 * (i >> 1) + 8 * (i & 1));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();                        // (the rows' sums go where q and the scales are)
+  } else {
+    const bf16* qp = p.q + ((size_t)q_tok * p.Hq + kvh * G + min(r, G - 1)) * D + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const bf16x8*>(qp + 64 * (i >> 1) + 8 * (i & 1));
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = r < G ? q[i] : bf16x8{};
   Row st;
 #pragma unroll
   for (int i = 0; i < 8; ++i) st.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   st.m = -1e30f;
   st.l = 0.f;
   for (int t = t0, i = 0; t < end; t += 128, ++i) {
-    const int blk = __builtin_amdgcn_readlane(page, i);
-    if (blk < 0) continue;
-    Chunk c;
-    chunk_load(c, p, ((int64_t)blk * p.Hkv + kvh) * BS * D, t % BS);
-    const float ksc = lane_f(ks, i), vsc = lane_f(vs, i);
-    if (t + 32 <= end) chunk_take<false>(st, q, c, ksc, vsc, 32);
-    else chunk_take<true>(st, q, c, ksc, vsc, end - t);
+    const bool some = page_of(i) >= 0;
+    float x[8];
+    if (some) chunk_scores(x, q, c, lane_f(ks, i));
+    load_k(c, rsrc_of(p.k_cache, i + 1));
+    if (some) chunk_rows(st, x, c, lane_f(vs, i), end - t);
+    load_v(c, rsrc_of(p.v_cache, i + 1));
   }
   float l = st.l;
   l += __shfl_xor(l, 16, 64);
@@ -186,33 +377,65 @@ __global__ __launch_bounds__(256, 2) void scaled_decode_kernel(ScaledAttn p) {
     }
   }
   __syncthreads();
-  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 8;
-  if (row >= G) return;
-  float M = -1e30f, L = 0.f, acc[8] = {};
+  const bool alone = p.num_parts == 1 || (p.tickets != nullptr && nparts <= 1);
+  const bool past = p.tickets != nullptr && !alone;
+  // a thread's dims: 8 in a row, of partial rows that go past the caches 4 and 4, whole lines to a store
+  const int row = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (past ? 4 : 8), d4 = past ? 64 : 4;
+  if (row < G) {
+    float M = -1e30f, L = 0.f, acc[8] = {};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i * G + row]);
+    for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i * G + row]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float f = __builtin_amdgcn_exp2f(m_s[i * G + row] - M);
-    L += f * l_s[i * G + row];
+    for (int i = 0; i < 4; ++i) {
+      const float f = __builtin_amdgcn_exp2f(m_s[i * G + row] - M);
+      L += f * l_s[i * G + row];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += f * o_s[(i * G + row) * (D + 4) + d0 + j];
+      for (int j = 0; j < 8; ++j) acc[j] += f * o_s[(i * G + row) * (D + 4) + d0 + (j >> 2) * d4 + (j & 3)];
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const int64_t at = ((int64_t)(seq * p.Hkv + kvh) * p.num_parts + part) * G + row;
+    if (alone) {
+      bf16x8 o;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = f2bf(acc[j] * inv);
+      *reinterpret_cast<bf16x8*>(p.out + ((size_t)q_tok * p.Hq + kvh * G + row) * D + d0) = o;
+    } else if (past) {
+      const __amdgpu_buffer_rsrc_t rs =
+          __builtin_amdgcn_make_buffer_rsrc((void*)(p.part_o + (at - row) * D), (short)0, G * D * 4, 0x00020000);
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            u32x4{__float_as_uint(acc[4 * k] * inv), __float_as_uint(acc[4 * k + 1] * inv),
+                  __float_as_uint(acc[4 * k + 2] * inv), __float_as_uint(acc[4 * k + 3] * inv)},
+            rs, (row * D + d0 + 64 * k) * 4, 0, kPast);
+      if (d0 == 0) {
+        __hip_atomic_store(p.part_m + at, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(p.part_l + at, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p.part_o[at * D + d0 + j] = acc[j] * inv;
+      if (d0 == 0) {
+        p.part_m[at] = M;
+        p.part_l[at] = L;
+      }
+    }
   }
-  const float inv = L > 0.f ? 1.f / L : 0.f;
-  if (p.num_parts == 1) {
-    bf16x8 o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = f2bf(acc[j] * inv);
-    *reinterpret_cast<bf16x8*>(p.out + ((size_t)q_tok * p.Hq + kvh * G + row) * D + d0) = o;
-    return;
+  if (!past) return;
+  // The last of the row's partitions to get here merges them.  Its stores acknowledged, a workgroup adds its share to
+  // the row's ticket: 1, the first partition 1 - nparts, so that all of them together leave the zero that was there.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int* flag = reinterpret_cast<int*>(m_s);
+  if (threadIdx.x == 0) {
+    const int share = part == 0 ? 1 - nparts : 1;
+    *flag = __hip_atomic_fetch_add(p.tickets + (int64_t)(seq * p.Hkv + kvh) * kCtrStride, share, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT) + share == 0;
   }
-  const size_t at = ((size_t)(seq * p.Hkv + kvh) * p.num_parts + part) * G + row;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) p.part_o[at * D + d0 + j] = acc[j] * inv;
-  if ((threadIdx.x & 15) == 0) {
-    p.part_m[at] = M;
-    p.part_l[at] = L;
-  }
+  __syncthreads();
+  const bool last = *flag != 0;
+  __syncthreads();
+  if (last) merge<true>(p, seq, kvh, nparts, q_tok, lds);
 }
 
 // ------------------------------------------------------------------------------------------------- prompts
@@ -450,9 +673,20 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
 
 void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
   if (num_seqs == 0) return;
-  const size_t smem = (size_t)(4 * p.G * (D + 4) + 8 * p.G) * sizeof(float);
-  scaled_decode_kernel<<<dim3(num_seqs, p.Hkv, p.num_parts), 256, smem, s>>>(p);
-  if (p.num_parts > 1) scaled_merge_kernel<<<dim3(num_seqs, p.Hkv), 256, 0, s>>>(p);
+  // Coarser partitions than asked for, in whole ones: under 512 keys a wave has too few chunks to pay for the merge,
+  // and more than 64 of them cost it more than they give.
+  ScaledAttn q = p;
+  const int by = std::min(std::max((511 + p.part_size) / p.part_size, (p.num_parts + 63) / 64),
+                          kDecodeMaxPart / p.part_size);
+  q.part_size = p.part_size * by;
+  q.num_parts = (p.num_parts + by - 1) / by;
+  const size_t merging = q.num_parts > 1 ? 16 * (D + 4) : 0;
+  const size_t smem = std::max<size_t>(4 * p.G * (D + 4) + 8 * p.G, merging) * sizeof(float);
+  const dim3 grid(num_seqs, p.Hkv, q.num_parts);
+  if (p.qkv != nullptr) scaled_decode_kernel<true><<<grid, 256, smem, s>>>(q);
+  else scaled_decode_kernel<false><<<grid, 256, smem, s>>>(q);
+  if (q.num_parts > 1 && p.tickets == nullptr)
+    scaled_merge_kernel<<<dim3(num_seqs, p.Hkv), 256, merging * sizeof(float), s>>>(q);
 }
 
 void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, hipStream_t s) {

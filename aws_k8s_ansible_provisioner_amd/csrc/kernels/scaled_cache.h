@@ -63,4 +63,58 @@ __device__ __forceinline__ bf16x8 codes_wide(uint32_t lo, uint32_t hi, float sca
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Head rows in 16 lanes, dims 8 li .. + 7 to a lane.
+__device__ __forceinline__ float pair_half(float v) {    // row_ror:8: lane ^ 8, which holds the other half's dims
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, false));
+}
+// Norm (optional), then the rotation (optional) of dims d and d + 64 by c and s, in fp32 throughout.
+__device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const bf16x8& w, bool rotate, const f32x4 (&c)[2],
+                                            const f32x4 (&s)[2], int li, float eps) {
+  if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    ss += dpp_mov<0xB1>(ss);
+    ss += dpp_mov<0x4E>(ss);
+    ss += dpp_mov<0x141>(ss);
+    ss += dpp_mov<0x140>(ss);
+    const float inv = rsqrtf(ss * (1.f / 128) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * bf2f(w[e]);
+  }
+  if (rotate) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float t = pair_half(x[e]) * s[e >> 2][e & 3];
+      x[e] = x[e] * c[e >> 2][e & 3] + (li < 8 ? -t : t);
+    }
+  }
+}
+
+// The new exponent of a page and head, by N threads that hold the largest magnitude `most` of its new entries, which
+// begin at token `off`; where a page that was begun before needs a larger one its codes are rounded anew, and waited
+// for.
+template <int N>
+__device__ __forceinline__ int page_exp(float most, float* scale, uint8_t* codes, int off, int BS) {
+  const int lane = threadIdx.x & (N - 1);
+  int e = scale_exp(most);
+  if (off > 0) {
+    const int was = stored_exp(*scale);
+    if (e > was) {
+      const float ratio = exp_scale(max(was - e, -126));   // (126 halvings leave no code but 0)
+      u32x4* at = reinterpret_cast<u32x4*>(codes);
+      for (int i = lane; i < BS * 8; i += N) {
+        u32x4 w = at[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], ratio);
+        at[i] = w;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    e = max(e, was);
+  }
+  if (lane == 0) *scale = exp_scale(e);
+  return e;
+}
+
 }  // namespace akap

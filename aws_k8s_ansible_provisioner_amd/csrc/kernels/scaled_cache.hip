@@ -16,46 +16,15 @@ namespace {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int D = 128;
 
-__device__ __forceinline__ uint32_t pair_half(uint32_t v) {
-  // row_ror:8 in a 16-lane row: lane ^ 8, which holds the other half's dims
-  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, false);
-}
-__device__ __forceinline__ float row16(float v) {
-  v += dpp_mov<0xB1>(v);
-  v += dpp_mov<0x4E>(v);
-  v += dpp_mov<0x141>(v);
-  v += dpp_mov<0x140>(v);
-  return v;
-}
-
-// a head row's dims 8 li .. + 7 in 16 lanes: norm (w != nullptr), then the rotation of dims d and d + 64, in
-// 32 bits throughout
-__device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const bf16x8& w, const float* cs, int li,
-                                            float eps) {
-  if (norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-    const float inv = rsqrtf(row16(ss) * (1.f / D) + eps);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * bf2f(w[e]);
-  }
-  if (cs != nullptr) {
-    const f32x4* at = reinterpret_cast<const f32x4*>(cs + 8 * (li & 7));
-    const f32x4 c[2] = {at[0], at[1]}, s[2] = {at[16], at[17]};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __uint_as_float(pair_half(__float_as_uint(x[e])));
-      const float t = other * s[e >> 2][e & 3];
-      x[e] = x[e] * c[e >> 2][e & 3] + (li < 8 ? -t : t);
-    }
-  }
-}
-
-__device__ __forceinline__ const float* angles(const ScaledAppend& p, int t) {
-  if (!p.rope) return nullptr;
-  const int64_t pos = p.positions[t];
-  return p.cos_sin + (size_t)(pos < 0 ? 0 : pos < p.max_pos ? pos : p.max_pos - 1) * D;
+// cos and sin of a row's dims 8 (li & 7) .. + 7
+struct Angles {
+  f32x4 c[2], s[2];
+};
+__device__ __forceinline__ Angles angles(const ScaledAppend& p, int t, int li) {
+  const int64_t pos = p.rope ? p.positions[t] : 0;
+  const f32x4* at = reinterpret_cast<const f32x4*>(
+      p.cos_sin + (size_t)(pos < 0 ? 0 : pos < p.max_pos ? pos : p.max_pos - 1) * D + 8 * (li & 7));
+  return Angles{{at[0], at[1]}, {at[16], at[17]}};
 }
 
 // q: 16 lanes per row and four of its heads
@@ -71,43 +40,19 @@ __device__ __forceinline__ void append_q(const ScaledAppend& p, int block) {
 #pragma unroll
   for (int j = 0; j < kQHeads; ++j)
     raw[j] = *reinterpret_cast<const bf16x8*>(row + min(h0 + j, p.Hq - 1) * D);
-  const float* cs = angles(p, t);
+  const Angles a = angles(p, t, li);
   const bf16x8 w = p.q_w != nullptr ? *reinterpret_cast<const bf16x8*>(p.q_w + 8 * li) : bf16x8{};
 #pragma unroll
   for (int j = 0; j < kQHeads; ++j) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = bf2f(raw[j][e]);
-    norm_rotate(x, p.q_w != nullptr, w, cs, li, p.eps);
+    norm_rotate(x, p.q_w != nullptr, w, p.rope, a.c, a.s, li, p.eps);
     bf16x8 o;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = f2bf(x[e]);
     if (h0 + j < p.Hq) *reinterpret_cast<bf16x8*>(p.q_out + ((size_t)t * p.Hq + h0 + j) * D + 8 * li) = o;
   }
-}
-
-// The new exponent of the run's page and head: `most` is the run's, uniform; where a page that was begun
-// before needs a larger one its codes are rounded anew, and waited for.
-__device__ __forceinline__ int page_exp(float most, float* scale, uint8_t* codes, int off, int BS) {
-  const int lane = threadIdx.x & 63;
-  int e = scale_exp(most);
-  if (off > 0) {
-    const int was = stored_exp(*scale);
-    if (e > was) {
-      const float ratio = exp_scale(max(was - e, -126));   // (126 halvings leave no code but 0)
-      u32x4* at = reinterpret_cast<u32x4*>(codes);
-      for (int i = lane; i < BS * D / 16; i += 64) {
-        u32x4 w = at[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], ratio);
-        at[i] = w;
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    e = max(e, was);
-  }
-  if (lane == 0) *scale = exp_scale(e);
-  return e;
 }
 
 // Keys of a run: rows t .. t + n - 1 into the page from token `off` on.  16 lanes per token, 4 J tokens at a
@@ -132,7 +77,8 @@ __device__ __forceinline__ void append_keys(const ScaledAppend& p, int h, int t,
     for (int j = 0; j < J; ++j) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[j][e] = bf2f(raw[j][e]);
-      norm_rotate(x[j], p.k_w != nullptr, w, angles(p, row[j]), li, p.eps);
+      const Angles a = angles(p, row[j], li);
+      norm_rotate(x[j], p.k_w != nullptr, w, p.rope, a.c, a.s, li, p.eps);
     }
   };
   float most = 0.f;
@@ -143,7 +89,7 @@ __device__ __forceinline__ void append_keys(const ScaledAppend& p, int h, int t,
 #pragma unroll
       for (int e = 0; e < 8; ++e) most = fmaxf(most, scale_mag(x[j][e]));
   }
-  const float inv = exp_scale(-page_exp(wave_max_dpp(most), p.k_scale + (size_t)blk * p.Hkv + h, codes, off, p.BS));
+  const float inv = exp_scale(-page_exp<64>(wave_max_dpp(most), p.k_scale + (size_t)blk * p.Hkv + h, codes, off, p.BS));
   for (int piece = 0; piece < pieces; ++piece) {
     if (pieces > 1) load(piece);
 #pragma unroll
@@ -178,7 +124,7 @@ __device__ __forceinline__ void append_values(const ScaledAppend& p, int h, int 
 #pragma unroll
     for (int j = 0; j < Q * 8; ++j) most = fmaxf(most, fmaxf(scale_mag(bf2f(x[j][0])), scale_mag(bf2f(x[j][1]))));
   }
-  const float inv = exp_scale(-page_exp(wave_max_dpp(most), p.v_scale + (size_t)blk * p.Hkv + h, codes, off, p.BS));
+  const float inv = exp_scale(-page_exp<64>(wave_max_dpp(most), p.v_scale + (size_t)blk * p.Hkv + h, codes, off, p.BS));
   for (int piece = 0; piece < pieces; ++piece) {
     if (pieces > 1) load(piece);
 #pragma unroll

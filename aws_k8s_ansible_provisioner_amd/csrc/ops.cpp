@@ -332,7 +332,8 @@ static void check_scaled(const Tensor& k_cache, const Tensor& v_cache, const Ten
   CHECK_GPU(k_cache); CHECK_CONTIG(k_cache); CHECK_CONTIG(v_cache); CHECK_CONTIG(scales);
   TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
               "scaled cache: uint8 K and V (e4m3 codes)");
-  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(3) == 128, "scaled cache: K [NB, Hkv, BS, 128]");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(0) > 0 && k_cache.size(3) == 128,
+              "scaled cache: K [NB, Hkv, BS, 128]");
   TORCH_CHECK(k_cache.size(2) > 0 && k_cache.size(2) % 32 == 0, "scaled cache: block size must be a multiple of 32");
   TORCH_CHECK(v_cache.dim() == 5 && v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) &&
                   v_cache.size(2) * 8 == k_cache.size(2) && v_cache.size(3) == 128 && v_cache.size(4) == 8,
@@ -469,7 +470,6 @@ static void set_parts(akap::ScaledAttn& p, const Tensor& out, int64_t B, int64_t
   TORCH_CHECK(num_parts > 0 && num_parts < 65536 && part_size > 0 && part_size % 128 == 0 &&
                   part_size <= akap::kDecodeMaxPart,
               "part_size must be a multiple of 128, at most ", akap::kDecodeMaxPart);
-  TORCH_CHECK(num_parts == 1 || part_size % p.BS == 0, "partitions must hold whole blocks");
   TORCH_CHECK(B < (1LL << 31) && p.Hkv < 65536, "too many rows");
   p.num_parts = num_parts;
   p.part_size = part_size;
@@ -483,6 +483,13 @@ static void set_parts(akap::ScaledAttn& p, const Tensor& out, int64_t B, int64_t
   p.part_m = part_m.data_ptr<float>();
   p.part_l = part_l.data_ptr<float>();
   p.part_o = part_o.data_ptr<float>();
+  // in-launch merge: as for the other caches' decode (set_tickets)
+  if (!tickets) return;
+  TORCH_CHECK(tickets->scalar_type() == at::kInt && tickets->is_contiguous(), "tickets: contiguous int32");
+  check_same_device(out, {&*tickets});
+  if (tickets->numel() >= B * p.Hkv * akap::kCtrStride && (uintptr_t)p.part_o % 16 == 0 &&
+      num_parts * p.G * 128 * 4 < (1LL << 31))
+    p.tickets = tickets->data_ptr<int>();
 }
 
 void scaled_attention_decode(Tensor out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor scales,
@@ -503,6 +510,40 @@ void scaled_attention_decode(Tensor out, Tensor q, Tensor k_cache, Tensor v_cach
   }
   p.q = (const __bf16*)q.data_ptr();
   set_parts(p, out, B, num_parts, part_size, part_m, part_l, part_o, tickets);
+  const c10::DeviceGuard g(out.device());
+  akap::launch_scaled_decode(p, B, cur_stream());
+}
+
+// scaled_cache_append of one row per sequence and scaled_attention_decode in one launch
+void scaled_attention_decode_fused(Tensor out, Tensor qkv, Tensor k_cache, Tensor v_cache, Tensor scales,
+                                   Tensor block_tables, Tensor seq_lens, Tensor positions, Tensor slots,
+                                   Tensor cos_sin, std::optional<Tensor> q_w, std::optional<Tensor> k_w,
+                                   Tensor part_m, Tensor part_l, Tensor part_o, int64_t num_parts,
+                                   int64_t part_size, int64_t G, double scale, double eps,
+                                   std::optional<Tensor> tickets) {
+  auto p = scaled_params(out, k_cache, v_cache, scales, block_tables, seq_lens, G, scale);
+  TORCH_CHECK(G + 2 <= 16, "fused decode supports up to 14 q heads per kv head");
+  const int64_t B = seq_lens.numel();
+  check_rows(qkv, out.size(1) + 2 * k_cache.size(1));
+  TORCH_CHECK(qkv.size(0) >= B && out.size(0) >= B, "qkv / out: a row for each sequence");
+  check_angles(qkv, positions, cos_sin, B);
+  check_norm_weight(qkv, q_w);
+  check_norm_weight(qkv, k_w);
+  TORCH_CHECK(slots.scalar_type() == at::kLong && slots.is_contiguous() && slots.numel() >= B,
+              "slots: int64, one per row");
+  check_same_device(out, {&qkv, &slots});
+  set_parts(p, out, B, num_parts, part_size, part_m, part_l, part_o, tickets);
+  // (a page's scale is one work item's)
+  TORCH_CHECK(num_parts == 1 || part_size % p.BS == 0, "partitions must hold whole blocks");
+  p.qkv = (const __bf16*)qkv.data_ptr();
+  p.qkv_stride = qkv.stride(0);
+  p.positions = positions.data_ptr<int64_t>();
+  p.slots = slots.data_ptr<int64_t>();
+  p.cos_sin = cos_sin.data_ptr<float>();
+  p.max_pos = cos_sin.size(0);
+  p.q_w = q_w ? (const __bf16*)q_w->data_ptr() : nullptr;
+  p.k_w = k_w ? (const __bf16*)k_w->data_ptr() : nullptr;
+  p.eps = (float)eps;
   const c10::DeviceGuard g(out.device());
   akap::launch_scaled_decode(p, B, cur_stream());
 }
@@ -1568,6 +1609,11 @@ TORCH_LIBRARY(akap, m) {
       "Tensor block_tables, Tensor seq_lens, Tensor? q_start, Tensor(b!) part_m, Tensor(c!) part_l, "
       "Tensor(d!) part_o, int num_parts, int part_size, int G, float scale, Tensor(e!)? tickets=None) -> ()");
   m.def(
+      "scaled_attention_decode_fused(Tensor(a!) out, Tensor qkv, Tensor(b!) k_cache, Tensor(c!) v_cache, "
+      "Tensor(d!) scales, Tensor block_tables, Tensor seq_lens, Tensor positions, Tensor slots, Tensor cos_sin, "
+      "Tensor? q_w, Tensor? k_w, Tensor(e!) part_m, Tensor(f!) part_l, Tensor(g!) part_o, int num_parts, "
+      "int part_size, int G, float scale, float eps, Tensor(h!)? tickets=None) -> ()");
+  m.def(
       "scaled_attention_prefill(Tensor(a!) out, Tensor? q, Tensor? qkv, Tensor k_cache, Tensor v_cache, "
       "Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start, Tensor tile_seq, Tensor tile_row, "
       "Tensor? positions, Tensor? cos_sin, Tensor? q_w, int G, float scale, float eps, int tile_rows=128) -> ()");
@@ -1669,6 +1715,7 @@ TORCH_LIBRARY_IMPL(akap, CUDA, m) {
   m.impl("paged_attention_decode_fused", &paged_attention_decode_fused);
   m.impl("scaled_cache_append", &scaled_cache_append);
   m.impl("scaled_attention_decode", &scaled_attention_decode);
+  m.impl("scaled_attention_decode_fused", &scaled_attention_decode_fused);
   m.impl("scaled_attention_prefill", &scaled_attention_prefill);
   m.impl("sample", &sample);
   m.impl("apply_penalties", &apply_penalties);

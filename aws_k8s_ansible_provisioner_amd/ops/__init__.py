@@ -312,7 +312,7 @@ def _check_scaled(k_cache, v_cache, scales) -> None:
     """The checks of csrc/ops.cpp check_scaled for CPU tensors."""
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise RuntimeError("scaled cache: uint8 K and V (e4m3 codes)")
-    if k_cache.dim() != 4 or k_cache.shape[2] % 32 or k_cache.shape[3] % 32:
+    if k_cache.dim() != 4 or not k_cache.shape[0] or k_cache.shape[2] % 32 or k_cache.shape[3] % 32:
         raise RuntimeError("scaled cache: K [NB, Hkv, BS, D], block size a multiple of 32")
     NB, H, BS, D = k_cache.shape
     if tuple(v_cache.shape) != (NB, H, BS // 8, D, 8):
@@ -386,8 +386,7 @@ def scaled_attention_decode(out, q, k_cache, v_cache, scales, block_tables, seq_
                             scale: float, workspace=None, num_parts: int = 1, part_size: int = 512,
                             q_start=None):
     """paged_attention_decode over a scaled cache: one row per sequence (row q_start[b], or b) over its
-    seq_lens[b] keys.  num_parts * part_size must hold the longest sequence's keys, part_size whole blocks
-    where there are several.  A key of a block table entry outside the cache is left out; a row that sees no
+    seq_lens[b] keys.  num_parts * part_size must hold the longest sequence's keys.  A key of a block table entry outside the cache is left out; a row that sees no
     key is zero."""
     if _native(q):
         if workspace is None:
@@ -408,20 +407,33 @@ def scaled_attention_decode(out, q, k_cache, v_cache, scales, block_tables, seq_
     return out
 
 
-def _check_parts(k_cache, num_parts: int, part_size: int) -> None:
+def _check_parts(k_cache, num_parts: int, part_size: int, whole: bool = False) -> None:
     if num_parts <= 0 or part_size <= 0 or part_size % 128 or part_size > DECODE_MAX_PART:
         raise RuntimeError(f"part_size must be a multiple of 128, at most {DECODE_MAX_PART}")
-    if num_parts > 1 and part_size % k_cache.shape[2]:
+    if whole and num_parts > 1 and part_size % k_cache.shape[2]:
         raise RuntimeError("partitions must hold whole blocks")
 
 
 def scaled_attention_decode_fused(out, qkv, k_cache, v_cache, scales, block_tables, seq_lens, positions,
                                   slots, cos_sin, q_w, k_w, gqa_group: int, scale: float, eps: float,
                                   workspace=None, num_parts: int = 1, part_size: int = 512):
-    """A decode step over a scaled cache from the projection's rows: scaled_cache_append of one new token per
-    sequence, then scaled_attention_decode of its normed and rotated q (as bf16).  out [B, Hq, D]."""
+    """A decode step over a scaled cache from the projection's rows, in one launch: scaled_cache_append of one
+    new token per sequence, then scaled_attention_decode of its normed and rotated q (as bf16).  out [B, Hq, D].
+    slots[b] is the place of key seq_lens[b] - 1 (or none: negative; nothing is appended to a sequence of no
+    keys); partitions hold whole blocks."""
     B, Hq, D = out.shape
     Hkv = k_cache.shape[1]
+    if gqa_group <= 14 and _native(qkv):
+        if workspace is None:
+            workspace = _decode_workspace(seq_lens.numel(), Hkv, gqa_group, num_parts, qkv.device)
+        pm, pl, po = workspace
+        torch.ops.akap.scaled_attention_decode_fused(out, qkv, k_cache, v_cache, scales, block_tables, seq_lens,
+                                                     positions, slots, cos_sin, q_w, k_w, pm, pl, po, num_parts,
+                                                     part_size, gqa_group, scale, eps,
+                                                     getattr(workspace, "tickets", None))
+        return out
+    _check_parts(k_cache, num_parts, part_size, whole=True)
+    slots = torch.where(seq_lens[:B] > 0, slots[:B], -1)
     q = torch.empty_like(out)
     scaled_cache_append(qkv[:B], q, k_cache, v_cache, scales, positions, slots, cos_sin, q_w, k_w, Hq, Hkv,
                         eps, True, decode=True)
