@@ -455,23 +455,113 @@ __device__ __forceinline__ float half_sum(float x) {
 __device__ __forceinline__ int row_key(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
 
 constexpr int kKeys = 64;
+constexpr int kSplitTiles = 8;     // key tiles that a part of a split tile takes at least
 
+// key tiles of a tile's rows, and the parts that they are cut into
+struct Tile {
+  int seq, row0, q0, q_len, ctx, keys, ntiles, parts;
+};
+template <int ROWS>
+__device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int tile) {
+  Tile t;
+  t.seq = __builtin_amdgcn_readfirstlane(p.tile_seq[tile]);
+  t.row0 = __builtin_amdgcn_readfirstlane(p.tile_row[tile]);
+  t.q0 = p.q_start[t.seq];
+  t.q_len = p.q_start[t.seq + 1] - t.q0;
+  t.ctx = p.seq_lens[t.seq] - t.q_len;
+  t.keys = keys_of(p, t.seq);
+  const int last = min(t.q_len - 1, (t.row0 + ROWS - 1) / p.G);
+  t.ntiles = last < 0 ? 0 : max(0, min(t.ctx + last, t.keys - 1) + kKeys) / kKeys;
+  t.parts = max(1, min(p.num_parts, t.ntiles / kSplitTiles));
+  return t;
+}
+
+// Scores of the next key tile are formed between the weights of this one, so that the matrix cores work beside the
+// exponentials: K of tile t + 1 and V of tile t are in LDS, K of t + 2 and V of t + 1 on their way.
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p) {
   constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
-  __shared__ __attribute__((aligned(16))) bf16 lds[2][2][kKeys * D];    // [buffer][K | V]
+  __shared__ __attribute__((aligned(16))) bf16 lds[2][2][kKeys * D];    // [K | V][buffer]
   const int flat = gridDim.x - 1 - blockIdx.x;     // the map rises by work: longest tiles first
-  const int tile = flat / p.Hkv, kvh = flat - tile * p.Hkv;
+  const int item = flat / p.Hkv, kvh = flat - item * p.Hkv;
+  const int tile = item / p.num_parts, part = item - tile * p.num_parts;
+  const Tile T = tile_of<ROWS>(p, tile);
+  if (part >= T.parts) return;
+  const int ta = T.ntiles * part / T.parts, tb = T.ntiles * (part + 1) / T.parts;
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int seq = __builtin_amdgcn_readfirstlane(p.tile_seq[tile]);
-  const int q0 = p.q_start[seq], q_len = p.q_start[seq + 1] - q0;
-  const int ctx = p.seq_lens[seq] - q_len, keys = keys_of(p, seq);
-  const int G = p.G, BS = p.BS, row0 = p.tile_row[tile];
+  const int G = p.G, BS = p.BS, row0 = T.row0, q0 = T.q0, keys = T.keys;
   const int R = row0 + 32 * w + r, pos = R / G, hig = R - pos * G;
-  const bool valid = pos < q_len;
-  const int limit = valid ? min(ctx + pos, keys - 1) : -1;
+  const bool valid = pos < T.q_len;
+  const int limit = valid ? min(T.ctx + pos, keys - 1) : -1;
+  const int w_first = (row0 + 32 * w) / G;
+  const bool active = w_first < T.q_len;
+  const int w_min = min(T.ctx + w_first, keys - 1);
 
+  // pieces: 512 of K and 512 of V to a tile; a wave's lie in one 32-key chunk
+  const int chunk = (w * PW * 64) >> 8;
+  const __attribute__((address_space(4))) int* bt =
+      (const __attribute__((address_space(4))) int*)(p.block_tables + (size_t)T.seq * p.bt_stride);
+  const __attribute__((address_space(4))) float* ksc = (const __attribute__((address_space(4))) float*)p.k_scale;
+  const __attribute__((address_space(4))) float* vsc = (const __attribute__((address_space(4))) float*)p.v_scale;
+  // the page of a 32-key chunk, -1 where it lies behind the keys or outside the cache
+  struct Pages {
+    int c[2];
+  };
+  auto pages_of = [&](int t) {
+    Pages g;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = 2 * t + k;
+      const int b = bt[32 * c < keys && t < tb ? 32 * c / BS : 0];
+      g.c[k] = 32 * c < keys && t < tb && (uint32_t)b < (uint32_t)p.num_blocks ? b : -1;
+    }
+    return g;
+  };
+  auto mine = [&](const Pages& g) { return chunk ? g.c[1] : g.c[0]; };
+  auto at_of = [&](int b, int t) {
+    return ((int64_t)max(b, 0) * p.Hkv + kvh) * BS * D + (int64_t)(32 * (2 * t + chunk) % BS) * D;
+  };
+  u32x4 kc[PW], vc[PW];
+  auto fetch = [&](u32x4 (&to)[PW], const uint8_t* cache, int b, int t) {
+    const __amdgpu_buffer_rsrc_t rs = chunk_rsrc(cache, at_of(b, t), b >= 0);    // (of no page: zeros)
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      to[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ((tid * PW + i) & 255) * 16, 0, 0));
+  };
+  // K image: token rows of 256 bytes, 16-byte column c of row k at c ^ (k & 15); V image: the groups as they are
+  auto store_k = [&](int buf, float scale) {
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int pc = (tid * PW + i) & 255;       // K: [half 2][dims / 32 4][row 16][2]
+      const int col = 4 * ((pc >> 5) & 3) + 2 * (pc & 1), r16 = (pc >> 1) & 15;
+      const int key = 32 * chunk + 8 * (r16 >> 2) + 4 * (pc >> 7) + (r16 & 3);
+      bf16* kl = lds[0][buf] + key * D;
+      *reinterpret_cast<bf16x8*>(kl + (col ^ (key & 15)) * 8) = codes_wide(kc[i][0], kc[i][1], scale);
+      *reinterpret_cast<bf16x8*>(kl + ((col + 1) ^ (key & 15)) * 8) = codes_wide(kc[i][2], kc[i][3], scale);
+    }
+  };
+  auto store_v = [&](int buf, float scale, int t) {
+    const int c = 2 * t + chunk;
+    if (32 * c + 32 > keys) {      // values behind the last key may be no numbers: zeros
+#pragma unroll
+      for (int i = 0; i < PW; ++i) {
+        const int left = keys - 32 * c - 8 * (((tid * PW + i) & 255) >> 6);
+        const uint32_t lo = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+        const uint32_t hi = left >= 8 ? ~0u : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1;
+        vc[i] = u32x4{vc[i][0] & lo, vc[i][1] & hi, vc[i][2] & lo, vc[i][3] & hi};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      bf16* vl = lds[1][buf] + (chunk * 256 + ((tid * PW + i) & 255)) * 16;
+      *reinterpret_cast<bf16x8*>(vl) = codes_wide(vc[i][0], vc[i][1], scale);
+      *reinterpret_cast<bf16x8*>(vl + 8) = codes_wide(vc[i][2], vc[i][3], scale);
+    }
+  };
+
+  Pages g0 = pages_of(ta), g1 = pages_of(ta + 1), g2 = pages_of(ta + 2);
+  fetch(kc, p.k_cache, mine(g0), ta);
   // Q^T: lane (r, h) holds dims 16 s + 8 h .. + 7 of its row
   bf16x8 qf[8];
   {
@@ -513,123 +603,77 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
         }
     }
   }
+  float ks = ksc[(int64_t)max(mine(g0), 0) * p.Hkv + kvh], vs = vsc[(int64_t)max(mine(g0), 0) * p.Hkv + kvh];
+  store_k(ta & 1, ks);
+  fetch(kc, p.k_cache, mine(g1), ta + 1);
+  fetch(vc, p.v_cache, mine(g0), ta);
+  __syncthreads();
 
-  const int last_pos = min(q_len - 1, (row0 + ROWS - 1) / G);
-  const int ntiles = last_pos < 0 ? 0 : (min(ctx + last_pos, keys - 1) + kKeys) / kKeys;
-  const int w_first = (row0 + 32 * w) / G;
-  const bool active = w_first < q_len;
-  const int w_limit = ctx + min(q_len - 1, (row0 + 32 * w + 31) / G), w_min = min(ctx + w_first, keys - 1);
-
-  // pieces: 512 of K and 512 of V to a tile; a wave's lie in one 32-key chunk
-  const int* bt = p.block_tables + (size_t)seq * p.bt_stride;
-  const int chunk = (w * PW * 64) >> 8;
-  u32x4 kc[PW], vc[PW];
-  float ks = 1.f, vs = 1.f;
-  // a chunk's page, or -1 where it lies behind the keys or outside the cache
-  auto page_of = [&](int c) -> int {
-    if (32 * c >= keys) return -1;
-    const int b = bt[32 * c / BS];
-    return (uint32_t)b < (uint32_t)p.num_blocks ? b : -1;
-  };
-  auto fetch = [&](int t) {
-    const int c = 2 * t + chunk, b = __builtin_amdgcn_readfirstlane(page_of(c));
-    if (b < 0) {
-#pragma unroll
-      for (int i = 0; i < PW; ++i) kc[i] = vc[i] = u32x4{0, 0, 0, 0};
-      return;
-    }
-    const int64_t at = ((int64_t)b * p.Hkv + kvh) * BS * D + (int64_t)(32 * c % BS) * D;
-    ks = p.k_scale[(size_t)b * p.Hkv + kvh];
-    vs = p.v_scale[(size_t)b * p.Hkv + kvh];
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      const int pc = (tid * PW + i) & 255;
-      kc[i] = *reinterpret_cast<const u32x4*>(p.k_cache + at + pc * 16);
-      vc[i] = *reinterpret_cast<const u32x4*>(p.v_cache + at + pc * 16);
-    }
-    if (32 * c + 32 > keys) {      // values behind the last key may be no numbers: zeros
-#pragma unroll
-      for (int i = 0; i < PW; ++i) {
-        const int mine = keys - 32 * c - 8 * (((tid * PW + i) & 255) >> 6);
-        const uint32_t lo = mine >= 4 ? ~0u : mine <= 0 ? 0u : (1u << (8 * mine)) - 1;
-        const uint32_t hi = mine >= 8 ? ~0u : mine <= 4 ? 0u : (1u << (8 * (mine - 4))) - 1;
-        vc[i] = u32x4{vc[i][0] & lo, vc[i][1] & hi, vc[i][2] & lo, vc[i][3] & hi};
-      }
-    }
-  };
-  // K image: token rows of 256 bytes, 16-byte column c of row k at c ^ (k & 15); V image: the groups as they are
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      const int pc = (tid * PW + i) & 255;       // K: [half 2][dims / 32 4][row 16][2]
-      const int col = 4 * ((pc >> 5) & 3) + 2 * (pc & 1), r16 = (pc >> 1) & 15;
-      const int key = 32 * chunk + 8 * (r16 >> 2) + 4 * (pc >> 7) + (r16 & 3);
-      bf16* kl = lds[buf][0] + key * D;
-      *reinterpret_cast<bf16x8*>(kl + (col ^ (key & 15)) * 8) = codes_wide(kc[i][0], kc[i][1], ks);
-      *reinterpret_cast<bf16x8*>(kl + ((col + 1) ^ (key & 15)) * 8) = codes_wide(kc[i][2], kc[i][3], ks);
-      bf16* vl = lds[buf][1] + (chunk * 256 + pc) * 16;
-      *reinterpret_cast<bf16x8*>(vl) = codes_wide(vc[i][0], vc[i][1], vs);
-      *reinterpret_cast<bf16x8*>(vl + 8) = codes_wide(vc[i][2], vc[i][3], vs);
-    }
-  };
-
-  f32x16 o[4];
+  f32x16 o[4], s[2];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   float m = -1e30f, l = 0.f;
-  if (ntiles > 0) {
-    fetch(0);
-    store(0);
-  }
+  auto scores = [&](f32x16 (&to)[2], int buf) {
+    const bf16* kl = lds[0][buf];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) to[k][j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int key = 32 * k + row_key(r);
+        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kl + key * D + ((2 * i + h) ^ (key & 15)) * 8);
+        to[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i], to[k], 0, 0, 0);
+      }
+  };
+  if (active) scores(s, ta & 1);
+  store_v(ta & 1, vs, ta);
+  ks = ksc[(int64_t)max(mine(g1), 0) * p.Hkv + kvh];
+  vs = vsc[(int64_t)max(mine(g1), 0) * p.Hkv + kvh];
+  store_k((ta + 1) & 1, ks);
   __syncthreads();
-  for (int t = 0; t < ntiles; ++t) {
-    const bool more = t + 1 < ntiles;
-    if (more) fetch(t + 1);
-    const int key0 = t * kKeys;
-    if (active && key0 <= w_limit) {
-      const bf16* kl = lds[t & 1][0];
-      const bf16* vl = lds[t & 1][1];
-      f32x16 s[2];
+  for (int t = ta; t < tb; ++t) {
+    // (behind the last tile's: zeros, of which nothing is made)
+    fetch(kc, p.k_cache, mine(g2), t + 2);
+    fetch(vc, p.v_cache, mine(g1), t + 1);
+    const Pages g3 = pages_of(t + 3);
+    ks = ksc[(int64_t)max(mine(g2), 0) * p.Hkv + kvh];
+    const float vs2 = vsc[(int64_t)max(mine(g2), 0) * p.Hkv + kvh];
+    if (active) {
+      const int key0 = t * kKeys;
+      // mask and maximum, on the raw scores
+      float top = -INFINITY;
+      if (key0 + kKeys - 1 > w_min || g0.c[0] < 0 || g0.c[1] < 0) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || g0.c[k] < 0) s[k][j] = -INFINITY;
+      }
+      f32x16 sn[2];
+      scores(sn, (t + 1) & 1);
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[k][j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int key = 32 * k + row_key(r);
-          const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kl + key * D + ((2 * i + h) ^ (key & 15)) * 8);
-          s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i], s[k], 0, 0, 0);
-        }
-      const bool lost0 = page_of(2 * t) < 0, lost1 = page_of(2 * t + 1) < 0;    // uniform
-      float top = -INFINITY;
-      if (key0 + kKeys - 1 > w_min || lost0 || lost1) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || (k ? lost1 : lost0)) s[k][j] = -INFINITY;
-            top = fmaxf(top, s[k][j]);
-          }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) top = fmaxf(top, s[k][j]);
-      }
-      const float mn = fmaxf(m, half_max(top) * p.scale_log2), a = __builtin_amdgcn_exp2f(m - mn);
-      float sum = 0.f;
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, s[k][j]);
+      // the maximum moves, and sums are scaled, only where it is exceeded by 2^8: weights up to that are as good
+      const float cand = fmaxf(m, half_max(top) * p.scale_log2), mn = cand > m + 8.f ? cand : m;
+      const float a = __builtin_amdgcn_exp2f(m - mn);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      bf16x8 pb[2][2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          s[k][j] = __builtin_amdgcn_exp2f(fmaf(s[k][j], p.scale_log2, -mn));
-          sum += s[k][j];
+          const float e = __builtin_amdgcn_exp2f(fmaf(s[k][j], p.scale_log2, -mn));
+          sum[j & 3] += e;
+          pb[k][j >> 3][j & 7] = f2bf(e);
         }
-      l = l * a + half_sum(sum);
+      l = l * a + half_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
       if (__any(mn != m)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -637,24 +681,43 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
           for (int j = 0; j < 16; ++j) o[i][j] *= a;
       }
       m = mn;
+      const bf16* vl = lds[1][t & 1];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-          bf16x8 pb;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) pb[j] = f2bf(s[k][8 * s2 + j]);
+        for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
           for (int dt = 0; dt < 4; ++dt) {
             const bf16x8 vf = *reinterpret_cast<const bf16x8*>(vl + ((4 * k + 2 * s2 + h) * D + 32 * dt + r) * 8);
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb, o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[k][s2], o[dt], 0, 0, 0);
           }
-        }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) s[k] = sn[k];
     }
-    if (more) store((t + 1) & 1);
+    store_k(t & 1, ks);
+    store_v((t + 1) & 1, vs, t + 1);
+    vs = vs2;
+    g0 = g1;
+    g1 = g2;
+    g2 = g3;
     __syncthreads();
   }
   // dims 32 dt + 8 i + 4 h .. + 3 of a row to a lane
+  if (T.parts > 1) {
+    const int64_t at = ((int64_t)(tile * p.num_parts + part) * p.Hkv + kvh) * ROWS + 32 * w + r;
+    float* to = p.part_o + at * D + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(to + 32 * dt + 8 * i) =
+            f32x4{o[dt][4 * i], o[dt][4 * i + 1], o[dt][4 * i + 2], o[dt][4 * i + 3]};
+    if (h == 0) {
+      p.part_m[at] = m;
+      p.part_l[at] = l;
+    }
+    return;
+  }
   if (!valid) return;
   const float inv = l > 0.f ? 1.f / l : 0.f;
   bf16* to = p.out + ((size_t)(q0 + pos) * p.Hq + kvh * G + hig) * D + 4 * h;
@@ -667,6 +730,33 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
       for (int j = 0; j < 4; ++j) x[j] = f2bf(o[dt][4 * i + j] * inv);
       *reinterpret_cast<bf16x4*>(to + 32 * dt + 8 * i) = x;
     }
+}
+
+// The parts of split tiles: 32 threads to a row, 8 rows to a workgroup.
+template <int ROWS>
+__global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p) {
+  const int item = blockIdx.x / (ROWS / 8), sub = blockIdx.x - item * (ROWS / 8);
+  const int tile = item / p.Hkv, kvh = item - tile * p.Hkv;
+  const Tile T = tile_of<ROWS>(p, tile);
+  if (T.parts <= 1) return;
+  const int row = sub * 8 + (threadIdx.x >> 5), d0 = (threadIdx.x & 31) * 4;
+  const int R = T.row0 + row, pos = R / p.G;
+  if (pos >= T.q_len) return;
+  float M = -1e30f, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < T.parts; ++i) {
+    const int64_t at = ((int64_t)(tile * p.num_parts + i) * p.Hkv + kvh) * ROWS + row;
+    const float m = p.part_m[at], mn = fmaxf(M, m);
+    const float a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(m - mn);
+    acc = acc * a + *reinterpret_cast<const f32x4*>(p.part_o + at * D + d0) * b;
+    L = L * a + p.part_l[at] * b;
+    M = mn;
+  }
+  const float inv = L > 0.f ? 1.f / L : 0.f;
+  bf16x4 x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] = f2bf(acc[j] * inv);
+  *reinterpret_cast<bf16x4*>(p.out + ((size_t)(T.q0 + pos) * p.Hq + kvh * p.G + R - pos * p.G) * D + d0) = x;
 }
 
 }  // namespace
@@ -691,8 +781,13 @@ void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
 
 void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, hipStream_t s) {
   if (num_tiles == 0) return;
-  if (tile_rows == 256) scaled_prefill_kernel<8><<<num_tiles * p.Hkv, 512, 0, s>>>(p);
-  else scaled_prefill_kernel<4><<<num_tiles * p.Hkv, 256, 0, s>>>(p);
+  const int grid = num_tiles * p.Hkv * p.num_parts;
+  if (tile_rows == 256) scaled_prefill_kernel<8><<<grid, 512, 0, s>>>(p);
+  else scaled_prefill_kernel<4><<<grid, 256, 0, s>>>(p);
+  if (p.num_parts == 1) return;
+  const int merge = num_tiles * p.Hkv * (tile_rows / 8);
+  if (tile_rows == 256) scaled_prefill_merge_kernel<256><<<merge, 256, 0, s>>>(p);
+  else scaled_prefill_merge_kernel<128><<<merge, 256, 0, s>>>(p);
 }
 
 }  // namespace akap

@@ -552,7 +552,7 @@ void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional
                               Tensor v_cache, Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start,
                               Tensor tile_seq, Tensor tile_row, std::optional<Tensor> positions,
                               std::optional<Tensor> cos_sin, std::optional<Tensor> q_w, int64_t G, double scale,
-                              double eps, int64_t tile_rows) {
+                              double eps, int64_t tile_rows, int64_t parts, std::optional<Tensor> part) {
   auto p = scaled_params(out, k_cache, v_cache, scales, block_tables, seq_lens, G, scale);
   TORCH_CHECK(tile_rows == 128 || tile_rows == 256, "tile_rows must be 128 or 256");
   const int64_t B = seq_lens.numel();
@@ -560,7 +560,21 @@ void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional
     TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), "q_start / tile maps must be contiguous int32");
   TORCH_CHECK(q_start.numel() >= B + 1 && tile_row.numel() >= tile_seq.numel(), "q_start / tile maps too short");
   check_same_device(out, {&q_start, &tile_seq, &tile_row});
-  TORCH_CHECK(tile_seq.numel() * p.Hkv < (1LL << 31) && out.size(0) * G < (1LL << 31), "too many rows");
+  TORCH_CHECK(parts > 0 && tile_seq.numel() * p.Hkv * std::max<int64_t>(parts, 32) < (1LL << 31) &&
+                  out.size(0) * G < (1LL << 31),
+              "too many rows");
+  // split tiles: per (tile, part, kv head) and row 128 sums, then all rows' maxima, then all rows' sums
+  p.num_parts = parts;
+  if (parts > 1) {
+    const int64_t rows = tile_seq.numel() * parts * p.Hkv * tile_rows;
+    TORCH_CHECK(part && part->scalar_type() == at::kFloat && part->is_contiguous() && part->numel() >= rows * 130 &&
+                    (uintptr_t)part->data_ptr() % 16 == 0,
+                "parts of tiles: fp32 of 130 per row and part");
+    check_same_device(out, {&*part});
+    p.part_o = part->data_ptr<float>();
+    p.part_m = p.part_o + rows * 128;
+    p.part_l = p.part_m + rows;
+  }
   if (qkv) {
     TORCH_CHECK(positions && cos_sin, "rows of the projection need positions and cos_sin");
     check_rows(*qkv, out.size(1) + 2 * k_cache.size(1));
@@ -1616,7 +1630,8 @@ TORCH_LIBRARY(akap, m) {
   m.def(
       "scaled_attention_prefill(Tensor(a!) out, Tensor? q, Tensor? qkv, Tensor k_cache, Tensor v_cache, "
       "Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start, Tensor tile_seq, Tensor tile_row, "
-      "Tensor? positions, Tensor? cos_sin, Tensor? q_w, int G, float scale, float eps, int tile_rows=128) -> ()");
+      "Tensor? positions, Tensor? cos_sin, Tensor? q_w, int G, float scale, float eps, int tile_rows=128, "
+      "int parts=1, Tensor(b!)? part=None) -> ()");
   m.def(
       "sample(Tensor logits, Tensor temperature, Tensor top_k, Tensor top_p, Tensor seeds, "
       "Tensor steps, Tensor(a!) out_tokens, Tensor(b!) out_logprobs, "

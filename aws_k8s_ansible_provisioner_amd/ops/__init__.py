@@ -441,18 +441,34 @@ def scaled_attention_decode_fused(out, qkv, k_cache, v_cache, scales, block_tabl
                                    workspace, num_parts, part_size)
 
 
+def scaled_prefill_parts(grid: int, tile_rows: int, max_len: int) -> int:
+    """Parts along the keys that prompt tiles are cut into: as many as fill the card with one workgroup of
+    eight waves (tile_rows 256) or two of four to a CU, each of 512 keys or more."""
+    return max(1, min((512 if tile_rows == 128 else 256) // max(grid, 1), max_len // 512, 16))
+
+
 def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start, tile_seq,
-                             tile_row, gqa_group: int, scale: float, tile_rows: int = 128, qprep=None):
+                             tile_row, gqa_group: int, scale: float, tile_rows: int = 128, qprep=None,
+                             max_len: Optional[int] = None):
     """paged_attention_prefill over a scaled cache: causal attention of each sequence's rows q_start[b] ..
     q_start[b + 1] - 1, its last tokens, over its seq_lens[b] keys; the tile map as there (tile_rows 128 or
     256; sequences that no tile names are left as they are).
     qprep = (qkv, positions, cos_sin, q_w, eps): the kernel takes its q rows from the projection's, normed and
-    rotated by their positions, rounded to bf16 (q is not read then and may be None)."""
+    rotated by their positions, rounded to bf16 (q is not read then and may be None).
+    max_len: the longest sequence's keys where the host knows them (else what the block tables hold); a map of
+    few tiles over many keys is cut along the keys, by scratch of 520 bytes per row and part."""
     if _native(out):
+        parts = scaled_prefill_parts(tile_seq.numel() * k_cache.shape[1], tile_rows,
+                                     block_tables.shape[1] * k_cache.shape[2] if max_len is None else max_len)
+        part = None
+        if parts > 1:
+            part = torch.empty(tile_seq.numel() * k_cache.shape[1] * parts * tile_rows * 130,
+                               dtype=torch.float32, device=out.device)
         qkv, positions, cos_sin, q_w, eps = qprep if qprep is not None else (None, None, None, None, 0.0)
         torch.ops.akap.scaled_attention_prefill(out, None if qprep is not None else q, qkv, k_cache, v_cache,
                                                 scales, block_tables, seq_lens, q_start, tile_seq, tile_row,
-                                                positions, cos_sin, q_w, gqa_group, scale, eps, tile_rows)
+                                                positions, cos_sin, q_w, gqa_group, scale, eps, tile_rows,
+                                                parts, part)
         return out
     _check_scaled_attention(out, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group, scale)
     if tile_rows not in (64, 128, 256):
