@@ -91,29 +91,34 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const bf16
   }
 }
 
+// A page and head's codes rounded anew for a scale 2^-down times theirs, by N threads.
+template <int N>
+__device__ __forceinline__ void codes_grow(uint8_t* codes, int down, int BS) {
+  const float ratio = exp_scale(max(down, -126));      // (126 halvings leave no code but 0)
+  u32x4* at = reinterpret_cast<u32x4*>(codes);
+  for (int i = threadIdx.x & (N - 1); i < BS * 8; i += N) {
+    u32x4 w = at[i];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], ratio);
+    at[i] = w;
+  }
+}
+
 // The new exponent of a page and head, by N threads that hold the largest magnitude `most` of its new entries, which
 // begin at token `off`; where a page that was begun before needs a larger one its codes are rounded anew, and waited
 // for.
 template <int N>
 __device__ __forceinline__ int page_exp(float most, float* scale, uint8_t* codes, int off, int BS) {
-  const int lane = threadIdx.x & (N - 1);
   int e = scale_exp(most);
   if (off > 0) {
     const int was = stored_exp(*scale);
     if (e > was) {
-      const float ratio = exp_scale(max(was - e, -126));   // (126 halvings leave no code but 0)
-      u32x4* at = reinterpret_cast<u32x4*>(codes);
-      for (int i = lane; i < BS * 8; i += N) {
-        u32x4 w = at[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = codes_again(w[k], ratio);
-        at[i] = w;
-      }
+      codes_grow<N>(codes, was - e, BS);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     e = max(e, was);
   }
-  if (lane == 0) *scale = exp_scale(e);
+  if ((threadIdx.x & (N - 1)) == 0) *scale = exp_scale(e);
   return e;
 }
 

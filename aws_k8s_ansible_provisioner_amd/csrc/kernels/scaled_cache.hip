@@ -2,11 +2,10 @@
 // keys and values as codes of their page's scale (scaled_cache.h).
 //
 // A page's scale depends on all the entries that a call brings, and where it grows its old codes are rounded
-// anew, so a page and head belong to one wave: the one that holds the page's first row of the call.  Rows
-// whose slots follow each other inside a page are a run, its first row the leader; a wave looks over 32 rows
-// of the batch for leaders (over one row where rows are single tokens of their sequences) and takes each run,
-// its keys or its values: magnitudes first, then the codes, from registers where the run fits them.  The
-// caller keeps the rows of a page together, in rising slots.
+// anew, so a page and head belong to one workgroup, or a wave: the one that finds the page's first row of the call.
+// Rows whose slots follow each other inside a page are a run, its first row the leader; a workgroup looks over 32
+// rows of the batch for leaders (a wave over one, where rows are single tokens of their sequences) and takes each
+// run: magnitudes first, then the codes.  The caller keeps the rows of a page together, in rising slots.
 #include "scaled_cache.h"
 #include "kernels.h"
 
@@ -55,149 +54,236 @@ __device__ __forceinline__ void append_q(const ScaledAppend& p, int block) {
   }
 }
 
-// Keys of a run: rows t .. t + n - 1 into the page from token `off` on.  16 lanes per token, 4 J tokens at a
-// time, from a token that is a multiple of 4 on: four such tokens are 128-byte lines of the layout.
-template <int J>
+// dims 8 li .. + 7 of a row's key, normed and rotated
+__device__ __forceinline__ void key_row(float (&x)[8], const ScaledAppend& p, int h, int row, int li, const bf16x8& w) {
+  const bf16x8 raw = *reinterpret_cast<const bf16x8*>(p.qkv + (size_t)row * p.qkv_stride + (p.Hq + h) * D + 8 * li);
+  const Angles a = angles(p, row, li);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = bf2f(raw[e]);
+  norm_rotate(x, p.k_w != nullptr, w, p.rope, a.c, a.s, li, p.eps);
+}
+// four tokens from a multiple of 4 on are 128-byte lines of the layout
+__device__ __forceinline__ void put_key(uint8_t* codes, int o, int li, const float (&x)[8], float inv) {
+  *reinterpret_cast<u32x2*>(codes + k_swz_offset(o) + k_dim_offset(8 * li)) =
+      u32x2{codes4(x[0], x[1], x[2], x[3], inv), codes4(x[4], x[5], x[6], x[7], inv)};
+}
+// dims 2 lane and 2 lane + 1 of the 8 values from the run's first + `from` on (beyond the run: its first or last)
+__device__ __forceinline__ void value_rows(bf16x2 (&x)[8], const ScaledAppend& p, int h, int t, int n, int from, int lane) {
+  const bf16* src = p.qkv + (size_t)(p.Hq + p.Hkv + h) * D + 2 * lane;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    x[j] = *reinterpret_cast<const bf16x2*>(src + (size_t)(t + min(max(from + j, 0), n - 1)) * p.qkv_stride);
+}
+__device__ __forceinline__ float value_mag(const bf16x2 (&x)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, fmaxf(scale_mag(bf2f(x[j][0])), scale_mag(bf2f(x[j][1]))));
+  return m;
+}
+// the group of 8 tokens from o on, of which [off, off + n) are the run's
+__device__ __forceinline__ void put_values(uint8_t* codes, int o, int off, int n, int lane, const bf16x2 (&x)[8], float inv) {
+  u32x4 c;
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      c[2 * d + k] = codes4(bf2f(x[4 * k][d]), bf2f(x[4 * k + 1][d]), bf2f(x[4 * k + 2][d]), bf2f(x[4 * k + 3][d]), inv);
+  uint8_t* at = codes + (size_t)(o >> 3) * D * 8 + 16 * lane;
+  if (o >= off && o + 8 <= off + n) {
+    *reinterpret_cast<u32x4*>(at) = c;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (o + k >= off && o + k < off + n) {
+      at[k] = (uint8_t)(c[k >> 2] >> (8 * (k & 3)));
+      at[8 + k] = (uint8_t)(c[2 + (k >> 2)] >> (8 * (k & 3)));
+    }
+}
+
+// A run of a wave of its own, keys or values: rows t .. t + n - 1 (single tokens: one, as a rule) into the page from
+// token `off` on, 4 tokens of keys or 8 of values at a time.
 __device__ __forceinline__ void append_keys(const ScaledAppend& p, int h, int t, int n, int64_t blk, int off) {
   const int lane = threadIdx.x & 63, li = lane & 15, sub = lane >> 4;
   uint8_t* codes = p.k_cache + ((size_t)blk * p.Hkv + h) * p.BS * D;
-  const bf16* src = p.qkv + (size_t)(p.Hq + h) * D + 8 * li;
   const bf16x8 w = p.k_w != nullptr ? *reinterpret_cast<const bf16x8*>(p.k_w + 8 * li) : bf16x8{};
-  const int o0 = off & ~3, pieces = (off - o0 + n + 4 * J - 1) / (4 * J);
-  float x[J][8];
+  const int o0 = off & ~3, pieces = (off - o0 + n + 3) / 4;
+  float x[8];
   auto load = [&](int piece) {
-    bf16x8 raw[J];
-    int row[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      row[j] = t + min(max(o0 + (piece * J + j) * 4 + sub - off, 0), n - 1);
-      raw[j] = *reinterpret_cast<const bf16x8*>(src + (size_t)row[j] * p.qkv_stride);
-    }
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = bf2f(raw[j][e]);
-      const Angles a = angles(p, row[j], li);
-      norm_rotate(x[j], p.k_w != nullptr, w, p.rope, a.c, a.s, li, p.eps);
-    }
+    const int row = t + min(max(o0 + piece * 4 + sub - off, 0), n - 1);   // (beyond the run: its first or last again)
+    key_row(x, p, h, row, li, w);
   };
   float most = 0.f;
   for (int piece = 0; piece < pieces; ++piece) {
     load(piece);
 #pragma unroll
-    for (int j = 0; j < J; ++j)     // (rows beyond the run's are its first or last one again)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, scale_mag(x[j][e]));
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, scale_mag(x[e]));
   }
   const float inv = exp_scale(-page_exp<64>(wave_max_dpp(most), p.k_scale + (size_t)blk * p.Hkv + h, codes, off, p.BS));
   for (int piece = 0; piece < pieces; ++piece) {
     if (pieces > 1) load(piece);
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const int o = o0 + (piece * J + j) * 4 + sub;
-      const u32x2 c = {codes4(x[j][0], x[j][1], x[j][2], x[j][3], inv),
-                       codes4(x[j][4], x[j][5], x[j][6], x[j][7], inv)};
-      if (o >= off && o < off + n)
-        *reinterpret_cast<u32x2*>(codes + k_swz_offset(o) + k_dim_offset(8 * li)) = c;
-    }
+    const int o = o0 + piece * 4 + sub;
+    if (o >= off && o < off + n) put_key(codes, o, li, x, inv);
   }
 }
-
-// Values of a run: a lane holds dims 2 lane and 2 lane + 1 of 8 Q tokens, whole groups of the layout.
-template <int Q>
 __device__ __forceinline__ void append_values(const ScaledAppend& p, int h, int t, int n, int64_t blk, int off) {
   const int lane = threadIdx.x & 63;
   uint8_t* codes = p.v_cache + ((size_t)blk * p.Hkv + h) * p.BS * D;
-  const bf16* src = p.qkv + (size_t)(p.Hq + p.Hkv + h) * D + 2 * lane;
-  const int o0 = off & ~7, pieces = (off - o0 + n + 8 * Q - 1) / (8 * Q);
-  bf16x2 x[Q * 8];
-  auto load = [&](int piece) {
-#pragma unroll
-    for (int j = 0; j < Q * 8; ++j) {
-      const int row = t + min(max(o0 + piece * Q * 8 + j - off, 0), n - 1);
-      x[j] = *reinterpret_cast<const bf16x2*>(src + (size_t)row * p.qkv_stride);
-    }
-  };
+  const int o0 = off & ~7, pieces = (off - o0 + n + 7) / 8;
+  bf16x2 x[8];
   float most = 0.f;
   for (int piece = 0; piece < pieces; ++piece) {
-    load(piece);
-#pragma unroll
-    for (int j = 0; j < Q * 8; ++j) most = fmaxf(most, fmaxf(scale_mag(bf2f(x[j][0])), scale_mag(bf2f(x[j][1]))));
+    value_rows(x, p, h, t, n, o0 + piece * 8 - off, lane);
+    most = fmaxf(most, value_mag(x));
   }
   const float inv = exp_scale(-page_exp<64>(wave_max_dpp(most), p.v_scale + (size_t)blk * p.Hkv + h, codes, off, p.BS));
   for (int piece = 0; piece < pieces; ++piece) {
-    if (pieces > 1) load(piece);
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      const int o = o0 + (piece * Q + q) * 8;      // the group's first token
-      u32x4 c;
-#pragma unroll
-      for (int d = 0; d < 2; ++d)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          c[2 * d + k] = codes4(bf2f(x[8 * q + 4 * k][d]), bf2f(x[8 * q + 4 * k + 1][d]),
-                                bf2f(x[8 * q + 4 * k + 2][d]), bf2f(x[8 * q + 4 * k + 3][d]), inv);
-      uint8_t* at = codes + (size_t)(o >> 3) * D * 8 + 16 * lane;
-      if (o >= off && o + 8 <= off + n) {
-        *reinterpret_cast<u32x4*>(at) = c;
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (o + k >= off && o + k < off + n) {
-            at[k] = (uint8_t)(c[k >> 2] >> (8 * (k & 3)));
-            at[8 + k] = (uint8_t)(c[2 + (k >> 2)] >> (8 * (k & 3)));
-          }
-      }
-    }
+    if (pieces > 1) value_rows(x, p, h, t, n, o0 + piece * 8 - off, lane);
+    put_values(codes, o0 + piece * 8, off, n, lane, x, inv);
   }
 }
 
-// Rows [t0, t0 + rows) of the batch (rows <= 32), one head, keys or values: the runs that begin there.
-template <int ROWS>
-__device__ __forceinline__ void append_runs(const ScaledAppend& p, int t0, int h, bool values) {
+// A run of a workgroup: its keys and its values, a wave 8 tokens of every 32, both on their way at once; kept in
+// registers where the run fits kHeld such pieces (blocks of 32 tokens: one, of 64: two), else read a second time.  With a wave to
+// a run's keys or values, all of its tokens one after the other, a step of 1000 rows (8 kv heads) took 15 us, of 5000
+// rows in blocks of 64 (4 kv heads) 30.
+template <int kHeld>
+__device__ __forceinline__ void append_run(const ScaledAppend& p, int h, int t, int n, int64_t blk, int off,
+                                           float (*red)[4]) {
+  const int lane = threadIdx.x & 63, li = lane & 15, sub = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const size_t at = (size_t)blk * p.Hkv + h;
+  uint8_t *kcodes = p.k_cache + at * p.BS * D, *vcodes = p.v_cache + at * p.BS * D;
+  const bf16x8 kw = p.k_w != nullptr ? *reinterpret_cast<const bf16x8*>(p.k_w + 8 * li) : bf16x8{};
+  const int o0 = (off & ~7) + 8 * w, pieces = ((off & 7) + n + 31) / 32;
+  const int kwas = off > 0 ? stored_exp(p.k_scale[at]) : -100, vwas = off > 0 ? stored_exp(p.v_scale[at]) : -100;
+  float x[kHeld][2][8];
+  bf16x2 v[kHeld][8];
+  // a piece's tokens of this wave; of none: nothing
+  auto some = [&](int piece) { return o0 + 32 * piece + 8 > off && o0 + 32 * piece < off + n; };
+  auto load = [&](float (&k)[2][8], bf16x2 (&y)[8], int piece) {
+    const int o = o0 + 32 * piece;
+    value_rows(y, p, h, t, n, o - off, lane);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) key_row(k[j], p, h, t + min(max(o + 4 * j + sub - off, 0), n - 1), li, kw);
+  };
+  auto put = [&](const float (&k)[2][8], const bf16x2 (&y)[8], int piece, float kinv, float vinv) {
+    const int o = o0 + 32 * piece;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int at = o + 4 * j + sub;
+      if (at >= off && at < off + n) put_key(kcodes, at, li, k[j], kinv);
+    }
+    put_values(vcodes, o, off, n, lane, y, vinv);
+  };
+  float kmost = 0.f, vmost = 0.f;
+  auto count = [&](const float (&k)[2][8], const bf16x2 (&y)[8]) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kmost = fmaxf(kmost, scale_mag(k[j][e]));
+    vmost = fmaxf(vmost, value_mag(y));
+  };
+  const bool held = pieces <= kHeld;
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (some(i)) load(x[i], v[i], i);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (some(i)) count(x[i], v[i]);
+  } else {
+    for (int i = 0; i < pieces; ++i)
+      if (some(i)) {
+        load(x[0], v[0], i);
+        count(x[0], v[0]);
+      }
+  }
+  kmost = wave_max_dpp(kmost);
+  vmost = wave_max_dpp(vmost);
+  if (lane == 0) {
+    red[0][w] = kmost;
+    red[1][w] = vmost;
+  }
+  __syncthreads();
+  kmost = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  vmost = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+  const int ke = max(scale_exp(kmost), kwas), ve = max(scale_exp(vmost), vwas);
+
+  if (off > 0 && ke > kwas) codes_grow<256>(kcodes, kwas - ke, p.BS);
+  if (off > 0 && ve > vwas) codes_grow<256>(vcodes, vwas - ve, p.BS);
+  __syncthreads();      // (the codes rounded anew, before new ones; and `red` read, before the next run)
+  if (threadIdx.x == 0) {
+    p.k_scale[at] = exp_scale(ke);
+    p.v_scale[at] = exp_scale(ve);
+  }
+  const float kinv = exp_scale(-ke), vinv = exp_scale(-ve);
+  if (held) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (some(i)) put(x[i], v[i], i, kinv, vinv);
+  } else {
+    for (int i = 0; i < pieces; ++i)
+      if (some(i)) {
+        load(x[0], v[0], i);
+        put(x[0], v[0], i, kinv, vinv);
+      }
+  }
+}
+
+// Rows [t0, t0 + ROWS) of the batch (ROWS <= 32): `run` for each run that begins there.  The slots of 64 rows, one to a
+// lane, tell where runs begin and, as a rule, end.
+template <int ROWS, typename F>
+__device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F& run) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)p.num_blocks * p.BS;
+  const bool narrow = cap < (1ll << 31);
   auto slot_of = [&](int t) -> int64_t {
     const int64_t s = t >= 0 && t < p.T ? p.slots[t] : -1;
     return s < cap ? s : -1;        // (a slot outside the cache is no slot)
   };
-  const int t = t0 + lane;
-  const int64_t mine = lane < ROWS ? slot_of(t) : -1;
-  const int64_t before = lane < ROWS ? slot_of(t - 1) : -1;
-  uint64_t leaders = __ballot(mine >= 0 && (before != mine - 1 || before < 0 || mine % p.BS == 0));
+  const int64_t mine = slot_of(t0 + lane), before = slot_of(t0 + lane - 1);
+  const int64_t page = mine < 0 ? 0 : narrow ? (int64_t)((uint32_t)mine / (uint32_t)p.BS) : mine / p.BS;
+  const int off = (int)(mine - page * p.BS);
+  const bool follows = mine >= 0 && before == mine - 1 && off != 0;
+  const uint64_t on = __ballot(follows);
+  uint64_t leaders = __ballot(lane < ROWS && mine >= 0 && !follows);
   while (leaders != 0) {
     const int l = __builtin_ctzll(leaders);
     leaders &= leaders - 1;
-    const int64_t s = ((int64_t)__builtin_amdgcn_readlane((int)(mine >> 32), l) << 32) |
-                      (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
-    const int64_t blk = s / p.BS;
-    const int off = (int)(s % p.BS), room = p.BS - off;
-    int n = 1;                       // rows of the run: as far as the slots go on, inside the page
-    while (n < room) {
+    const int64_t blk = ((int64_t)__builtin_amdgcn_readlane((int)(page >> 32), l) << 32) |
+                        (uint32_t)__builtin_amdgcn_readlane((int)page, l);
+    const int o = __builtin_amdgcn_readlane(off, l);
+    int n = 1 + __builtin_ctzll(~(on >> 1 >> l));     // rows of the run (at most 64 - l)
+    while (l + n >= 64 && n < p.BS - o) {             // and of what follows the 64
       const int i = n + lane;
-      const uint64_t on = __ballot(i < room && slot_of(t0 + l + i) == s + i);
-      const int more = on == ~0ull ? 64 : __builtin_ctzll(~on);
-      n += more;
-      if (more < 64) break;
+      const uint64_t more = __ballot(i < p.BS - o && slot_of(t0 + l + i) == blk * p.BS + o + i);
+      n += more == ~0ull ? 64 : __builtin_ctzll(~more);
+      if (more != ~0ull) break;
     }
-    if (values) append_values<ROWS == 1 ? 1 : 4>(p, h, t0 + l, n, blk, off);
-    else append_keys<ROWS == 1 ? 1 : 8>(p, h, t0 + l, n, blk, off);
+    run(t0 + l, n, blk, o);
   }
 }
 
+template <int HELD>
 __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int single_blocks, int run_blocks) {
+  __shared__ float red[2][4];
   int b = blockIdx.x;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = 2 * p.Hkv;
   if (b < single_blocks) {
-    const int item = b * 4 + w;
-    if (item < p.singles * per) append_runs<1>(p, item / per, (item % per) >> 1, item & 1);
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = 2 * p.Hkv;
+    const int item = b * 4 + w, t = item / per, h = (item - t * per) >> 1;
+    if (t >= p.singles) return;
+    for_runs<1>(p, t, [&](int t, int n, int64_t blk, int off) {
+      if (item & 1) append_values(p, h, t, n, blk, off);
+      else append_keys(p, h, t, n, blk, off);
+    });
     return;
   }
   b -= single_blocks;
   if (b < run_blocks) {
-    const int item = b * 4 + w, t0 = p.singles + item / per * 32;
-    if (t0 < p.T) append_runs<32>(p, t0, (item % per) >> 1, item & 1);
+    const int span = b / p.Hkv, h = b - span * p.Hkv;
+    for_runs<32>(p, p.singles + 32 * span,
+                 [&](int t, int n, int64_t blk, int off) { append_run<HELD>(p, h, t, n, blk, off, red); });
     return;
   }
   append_q(p, b - run_blocks);
@@ -208,10 +294,12 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
 void launch_scaled_append(const ScaledAppend& p, hipStream_t s) {
   const long per = 2 * p.Hkv;
   const long single = (p.singles * per + 3) / 4;
-  const long runs = ((long)(p.T - p.singles + 31) / 32 * per + 3) / 4;
+  const long runs = (long)(p.T - p.singles + 31) / 32 * p.Hkv;
   const long q = ((long)p.q_rows * ((p.Hq + kQHeads - 1) / kQHeads) + 15) / 16;
   if (single + runs + q == 0) return;
-  scaled_append_kernel<<<dim3((unsigned)(single + runs + q)), 256, 0, s>>>(p, (int)single, (int)runs);
+  const dim3 grid((unsigned)(single + runs + q));
+  if (p.BS <= 32) scaled_append_kernel<1><<<grid, 256, 0, s>>>(p, (int)single, (int)runs);
+  else scaled_append_kernel<2><<<grid, 256, 0, s>>>(p, (int)single, (int)runs);
 }
 
 }  // namespace akap
