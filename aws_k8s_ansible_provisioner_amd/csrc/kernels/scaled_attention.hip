@@ -471,23 +471,27 @@ __device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int tile) {
   t.ctx = p.seq_lens[t.seq] - t.q_len;
   t.keys = keys_of(p, t.seq);
   const int last = min(t.q_len - 1, (t.row0 + ROWS - 1) / p.G);
-  t.ntiles = last < 0 ? 0 : max(0, min(t.ctx + last, t.keys - 1) + kKeys) / kKeys;
+  t.ntiles = last < 0 ? 0 : max(0, min(t.ctx + last, t.keys - 1)) / kKeys + 1;
   t.parts = max(1, min(p.num_parts, t.ntiles / kSplitTiles));
   return t;
 }
 
-// Scores of the next key tile are formed between the weights of this one, so that the matrix cores work beside the
-// exponentials: K of tile t + 1 and V of tile t are in LDS, K of t + 2 and V of t + 1 on their way.
+// A wave's step has two halves, with a barrier behind each: products (outputs of tile u by its weights, scores of tile
+// u + 1; beside them K of tile u + 2 and V of tile u + 1 are widened into LDS, where their buffers are free, and the
+// next ones asked for) and the weights of the next tile.  Of eight waves the later four go half a step behind: the two
+// waves of a SIMD are in different halves, one's products beside the other's exponentials.
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p) {
+  constexpr bool LATE = NW == 8;
   constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
   __shared__ __attribute__((aligned(16))) bf16 lds[2][2][kKeys * D];    // [K | V][buffer]
   const int flat = gridDim.x - 1 - blockIdx.x;     // the map rises by work: longest tiles first
-  const int item = flat / p.Hkv, kvh = flat - item * p.Hkv;
-  const int tile = item / p.num_parts, part = item - tile * p.num_parts;
+  const int item = __builtin_amdgcn_readfirstlane(flat / p.Hkv), kvh = flat - item * p.Hkv;
+  const int tile = __builtin_amdgcn_readfirstlane(item / p.num_parts), part = item - tile * p.num_parts;
   const Tile T = tile_of<ROWS>(p, tile);
-  if (part >= T.parts) return;
-  const int ta = T.ntiles * part / T.parts, tb = T.ntiles * (part + 1) / T.parts;
+  if (part >= T.parts || T.ntiles == 0) return;
+  const int ta = __builtin_amdgcn_readfirstlane(T.ntiles * part / T.parts);
+  const int tb = __builtin_amdgcn_readfirstlane(T.ntiles * (part + 1) / T.parts);
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.G, BS = p.BS, row0 = T.row0, q0 = T.q0, keys = T.keys;
@@ -495,36 +499,35 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
   const bool valid = pos < T.q_len;
   const int limit = valid ? min(T.ctx + pos, keys - 1) : -1;
   const int w_first = (row0 + 32 * w) / G;
-  const bool active = w_first < T.q_len;
   const int w_min = min(T.ctx + w_first, keys - 1);
 
   // pieces: 512 of K and 512 of V to a tile; a wave's lie in one 32-key chunk
   const int chunk = (w * PW * 64) >> 8;
-  const __attribute__((address_space(4))) int* bt =
-      (const __attribute__((address_space(4))) int*)(p.block_tables + (size_t)T.seq * p.bt_stride);
-  const __attribute__((address_space(4))) float* ksc = (const __attribute__((address_space(4))) float*)p.k_scale;
-  const __attribute__((address_space(4))) float* vsc = (const __attribute__((address_space(4))) float*)p.v_scale;
-  // the page of a 32-key chunk, -1 where it lies behind the keys or outside the cache
-  struct Pages {
-    int c[2];
+  // Pages and scales of 64 chunks, one to a lane, from tile `held` on; read by readlane, so that no step waits for
+  // the table.  A page is -1 where the chunk lies behind the keys or outside the cache.
+  int held = ta, page_l, off_l;
+  float ks_l, vs_l;
+  auto hold = [&](int t) {
+    held = t;
+    const int c = 2 * t + lane;
+    const bool some = 32 * c < keys && c < 2 * tb;
+    const int column = some ? 32 * c / BS : 0;
+    const int b = p.block_tables[(size_t)T.seq * p.bt_stride + column];
+    off_l = some ? (32 * c - column * BS) * D : 0;
+    page_l = some && (uint32_t)b < (uint32_t)p.num_blocks ? b : -1;
+    const int64_t at = (int64_t)max(page_l, 0) * p.Hkv + kvh;
+    ks_l = p.k_scale[at];
+    vs_l = p.v_scale[at];
   };
-  auto pages_of = [&](int t) {
-    Pages g;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int c = 2 * t + k;
-      const int b = bt[32 * c < keys && t < tb ? 32 * c / BS : 0];
-      g.c[k] = 32 * c < keys && t < tb && (uint32_t)b < (uint32_t)p.num_blocks ? b : -1;
-    }
-    return g;
-  };
-  auto mine = [&](const Pages& g) { return chunk ? g.c[1] : g.c[0]; };
-  auto at_of = [&](int b, int t) {
-    return ((int64_t)max(b, 0) * p.Hkv + kvh) * BS * D + (int64_t)(32 * (2 * t + chunk) % BS) * D;
-  };
+  hold(ta);
+  auto page_of = [&](int t, int k) { return __builtin_amdgcn_readlane(page_l, 2 * (t - held) + k); };
+  auto kscale_of = [&](int t) { return lane_f(ks_l, 2 * (t - held) + chunk); };
+  auto vscale_of = [&](int t) { return lane_f(vs_l, 2 * (t - held) + chunk); };
   u32x4 kc[PW], vc[PW];
-  auto fetch = [&](u32x4 (&to)[PW], const uint8_t* cache, int b, int t) {
-    const __amdgpu_buffer_rsrc_t rs = chunk_rsrc(cache, at_of(b, t), b >= 0);    // (of no page: zeros)
+  auto fetch = [&](u32x4 (&to)[PW], const uint8_t* cache, int t) {
+    const int i0 = 2 * (t - held) + chunk, b = __builtin_amdgcn_readlane(page_l, i0);
+    const __amdgpu_buffer_rsrc_t rs = chunk_rsrc(cache, ((int64_t)max(b, 0) * p.Hkv + kvh) * BS * D +
+                                                            __builtin_amdgcn_readlane(off_l, i0), b >= 0);    // (of no page: zeros)
 #pragma unroll
     for (int i = 0; i < PW; ++i)
       to[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ((tid * PW + i) & 255) * 16, 0, 0));
@@ -541,17 +544,19 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
       *reinterpret_cast<bf16x8*>(kl + ((col + 1) ^ (key & 15)) * 8) = codes_wide(kc[i][2], kc[i][3], scale);
     }
   };
-  auto store_v = [&](int buf, float scale, int t) {
+  // values behind the last key may be no numbers: zeros
+  auto clear_v = [&](int t) {
     const int c = 2 * t + chunk;
-    if (32 * c + 32 > keys) {      // values behind the last key may be no numbers: zeros
+    if (32 * c + 32 <= keys) return;
 #pragma unroll
-      for (int i = 0; i < PW; ++i) {
-        const int left = keys - 32 * c - 8 * (((tid * PW + i) & 255) >> 6);
-        const uint32_t lo = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
-        const uint32_t hi = left >= 8 ? ~0u : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1;
-        vc[i] = u32x4{vc[i][0] & lo, vc[i][1] & hi, vc[i][2] & lo, vc[i][3] & hi};
-      }
+    for (int i = 0; i < PW; ++i) {
+      const int left = keys - 32 * c - 8 * (((tid * PW + i) & 255) >> 6);
+      const uint32_t lo = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1;
+      const uint32_t hi = left >= 8 ? ~0u : left <= 4 ? 0u : (1u << (8 * (left - 4))) - 1;
+      vc[i] = u32x4{vc[i][0] & lo, vc[i][1] & hi, vc[i][2] & lo, vc[i][3] & hi};
     }
+  };
+  auto store_v = [&](int buf, float scale) {
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       bf16* vl = lds[1][buf] + (chunk * 256 + ((tid * PW + i) & 255)) * 16;
@@ -560,8 +565,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
     }
   };
 
-  Pages g0 = pages_of(ta), g1 = pages_of(ta + 1), g2 = pages_of(ta + 2);
-  fetch(kc, p.k_cache, mine(g0), ta);
+  fetch(kc, p.k_cache, ta);
+  fetch(vc, p.v_cache, ta);
+  u32x4 kc2[PW];
+  fetch(kc2, p.k_cache, ta + 1);
   // Q^T: lane (r, h) holds dims 16 s + 8 h .. + 7 of its row
   bf16x8 qf[8];
   {
@@ -603,11 +610,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
         }
     }
   }
-  float ks = ksc[(int64_t)max(mine(g0), 0) * p.Hkv + kvh], vs = vsc[(int64_t)max(mine(g0), 0) * p.Hkv + kvh];
-  store_k(ta & 1, ks);
-  fetch(kc, p.k_cache, mine(g1), ta + 1);
-  fetch(vc, p.v_cache, mine(g0), ta);
-  __syncthreads();
+  store_k(ta & 1, kscale_of(ta));
+  clear_v(ta);
+  store_v(ta & 1, vscale_of(ta));
+#pragma unroll
+  for (int i = 0; i < PW; ++i) kc[i] = kc2[i];
+  store_k((ta + 1) & 1, kscale_of(ta + 1));
+  fetch(kc, p.k_cache, ta + 2);
+  fetch(vc, p.v_cache, ta + 1);
 
   f32x16 o[4], s[2];
 #pragma unroll
@@ -615,63 +625,68 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   float m = -1e30f, l = 0.f;
-  auto scores = [&](f32x16 (&to)[2], int buf) {
-    const bf16* kl = lds[0][buf];
+  bf16x8 pb[4];                    // weights: keys 16 g + 8 h .. + 7
+  auto k_frag = [&](int buf, int i, int k) {
+    const int key = 32 * k + row_key(r);
+    return *reinterpret_cast<const bf16x8*>(lds[0][buf] + key * D + ((2 * i + h) ^ (key & 15)) * 8);
+  };
+  auto v_frag = [&](int buf, int g, int dt) {
+    return *reinterpret_cast<const bf16x8*>(lds[1][buf] + ((2 * g + h) * D + 32 * dt + r) * 8);
+  };
+  // (LDS alone: what is on its way from memory stays so)
+  auto half = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto scores = [&](int i, int buf) {
+    s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(buf, i >> 1, i & 1), qf[i >> 1], s[i & 1], 0, 0, 0);
+  };
+  auto rows = [&](int i, int buf) {
+    o[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(buf, i >> 2, i & 3), pb[i >> 2], o[i & 3], 0, 0, 0);
+  };
+  auto zero = [&]() {
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) to[k][j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int key = 32 * k + row_key(r);
-        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(kl + key * D + ((2 * i + h) ^ (key & 15)) * 8);
-        to[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[i], to[k], 0, 0, 0);
-      }
+      for (int j = 0; j < 16; ++j) s[k][j] = 0.f;
   };
-  if (active) scores(s, ta & 1);
-  store_v(ta & 1, vs, ta);
-  ks = ksc[(int64_t)max(mine(g1), 0) * p.Hkv + kvh];
-  vs = vsc[(int64_t)max(mine(g1), 0) * p.Hkv + kvh];
-  store_k((ta + 1) & 1, ks);
-  __syncthreads();
-  for (int t = ta; t < tb; ++t) {
-    // (behind the last tile's: zeros, of which nothing is made)
-    fetch(kc, p.k_cache, mine(g2), t + 2);
-    fetch(vc, p.v_cache, mine(g1), t + 1);
-    const Pages g3 = pages_of(t + 3);
-    ks = ksc[(int64_t)max(mine(g2), 0) * p.Hkv + kvh];
-    const float vs2 = vsc[(int64_t)max(mine(g2), 0) * p.Hkv + kvh];
-    if (active) {
-      const int key0 = t * kKeys;
-      // mask and maximum, on the raw scores
-      float top = -INFINITY;
-      if (key0 + kKeys - 1 > w_min || g0.c[0] < 0 || g0.c[1] < 0) {
+  const bool late = LATE && w >= 4;
+  half();
+  if (late) half();
+  zero();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) scores(i, ta & 1);
+  half();
+  // weights of tile u from its scores
+  auto weigh = [&](int u) {
+    {
+      const int t = u, key0 = t * kKeys;
+      const bool lost0 = page_of(t, 0) < 0, lost1 = page_of(t, 1) < 0;
+      if (key0 + kKeys - 1 > w_min || lost0 || lost1) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || g0.c[k] < 0) s[k][j] = -INFINITY;
+            if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || (k ? lost1 : lost0)) s[k][j] = -INFINITY;
       }
-      f32x16 sn[2];
-      scores(sn, (t + 1) & 1);
+      float tp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) top = fmaxf(top, s[k][j]);
+        for (int j = 0; j < 16; ++j) tp[j & 3] = fmaxf(tp[j & 3], s[k][j]);
+      const float top = fmaxf(fmaxf(tp[0], tp[1]), fmaxf(tp[2], tp[3]));
       // the maximum moves, and sums are scaled, only where it is exceeded by 2^8: weights up to that are as good
       const float cand = fmaxf(m, half_max(top) * p.scale_log2), mn = cand > m + 8.f ? cand : m;
       const float a = __builtin_amdgcn_exp2f(m - mn);
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
-      bf16x8 pb[2][2];
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const float e = __builtin_amdgcn_exp2f(fmaf(s[k][j], p.scale_log2, -mn));
           sum[j & 3] += e;
-          pb[k][j >> 3][j & 7] = f2bf(e);
+          pb[2 * k + (j >> 3)][j & 7] = f2bf(e);
         }
       l = l * a + half_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
       if (__any(mn != m)) {
@@ -681,27 +696,42 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
           for (int j = 0; j < 16; ++j) o[i][j] *= a;
       }
       m = mn;
-      const bf16* vl = lds[1][t & 1];
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-          for (int dt = 0; dt < 4; ++dt) {
-            const bf16x8 vf = *reinterpret_cast<const bf16x8*>(vl + ((4 * k + 2 * s2 + h) * D + 32 * dt + r) * 8);
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[k][s2], o[dt], 0, 0, 0);
-          }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) s[k] = sn[k];
     }
-    store_k(t & 1, ks);
-    store_v((t + 1) & 1, vs, t + 1);
-    vs = vs2;
-    g0 = g1;
-    g1 = g2;
-    g2 = g3;
-    __syncthreads();
+  };
+  for (int u = ta; u + 1 < tb; ++u) {
+    weigh(u);
+    clear_v(u + 1);
+    if (u + 3 - held > 31) hold(u);
+    half();
+    if constexpr (LATE) __builtin_amdgcn_s_setprio(1);
+    zero();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      scores(i, (u + 1) & 1);
+      rows(i, u & 1);
+    }
+    // (behind the last tile: zeros, of which nothing is made)
+    store_k(u & 1, kscale_of(u + 2));
+    store_v((u + 1) & 1, vscale_of(u + 1));
+    fetch(kc, p.k_cache, u + 3);
+    fetch(vc, p.v_cache, u + 2);
+    if constexpr (!LATE) {      // (keeps the four-wave form's registers: left to itself it spills 44 bytes)
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+      for (int i = 0; i < 12; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+      }
+    }
+    if constexpr (LATE) __builtin_amdgcn_s_setprio(0);
+    half();
   }
+  weigh(tb - 1);
+  half();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) rows(i, (tb - 1) & 1);
+  if (LATE && !late) half();
   // dims 32 dt + 8 i + 4 h .. + 3 of a row to a lane
   if (T.parts > 1) {
     const int64_t at = ((int64_t)(tile * p.num_parts + part) * p.Hkv + kvh) * ROWS + 32 * w + r;
