@@ -231,7 +231,8 @@ __device__ __forceinline__ void append_run(const ScaledAppend& p, int h, int t, 
   }
 }
 
-// Rows [t0, t0 + ROWS) of the batch (ROWS <= 32): `run` for each run that begins there.  The slots of 64 rows, one to a
+// Rows [t0, t0 + ROWS) of the batch (ROWS <= 32): `run` for each run that begins there, the i-th of
+// count.  The slots of 64 rows, one to a
 // lane, tell where runs begin and, as a rule, end.
 template <int ROWS, typename F>
 __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F& run) {
@@ -248,7 +249,8 @@ __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F&
   const bool follows = mine >= 0 && before == mine - 1 && off != 0;
   const uint64_t on = __ballot(follows);
   uint64_t leaders = __ballot(lane < ROWS && mine >= 0 && !follows);
-  while (leaders != 0) {
+  const int count = __popcll(leaders);
+  for (int i = 0; i < count; ++i) {
     const int l = __builtin_ctzll(leaders);
     leaders &= leaders - 1;
     const int64_t blk = ((int64_t)__builtin_amdgcn_readlane((int)(page >> 32), l) << 32) |
@@ -256,12 +258,12 @@ __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F&
     const int o = __builtin_amdgcn_readlane(off, l);
     int n = 1 + __builtin_ctzll(~(on >> 1 >> l));     // rows of the run (at most 64 - l)
     while (l + n >= 64 && n < p.BS - o) {             // and of what follows the 64
-      const int i = n + lane;
-      const uint64_t more = __ballot(i < p.BS - o && slot_of(t0 + l + i) == blk * p.BS + o + i);
+      const int at = n + lane;
+      const uint64_t more = __ballot(at < p.BS - o && slot_of(t0 + l + at) == blk * p.BS + o + at);
       n += more == ~0ull ? 64 : __builtin_ctzll(~more);
       if (more != ~0ull) break;
     }
-    run(t0 + l, n, blk, o);
+    run(i, count, t0 + l, n, blk, o);
   }
 }
 
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = 2 * p.Hkv;
     const int item = b * 4 + w, t = item / per, h = (item - t * per) >> 1;
     if (t >= p.singles) return;
-    for_runs<1>(p, t, [&](int t, int n, int64_t blk, int off) {
+    for_runs<1>(p, t, [&](int, int, int t, int n, int64_t blk, int off) {
       if (item & 1) append_values(p, h, t, n, blk, off);
       else append_keys(p, h, t, n, blk, off);
     });
@@ -282,8 +284,17 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
   b -= single_blocks;
   if (b < run_blocks) {
     const int span = b / p.Hkv, h = b - span * p.Hkv;
-    for_runs<32>(p, p.singles + 32 * span,
-                 [&](int t, int n, int64_t blk, int off) { append_run<HELD>(p, h, t, n, blk, off, red); });
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for_runs<32>(p, p.singles + 32 * span, [&](int i, int count, int t, int n, int64_t blk, int off) {
+      if (count <= 3) {
+        append_run<HELD>(p, h, t, n, blk, off, red);
+      } else if ((i & 3) == w) {
+        // Many short runs, a wave to each: 64 sequences of 3 tokens, 8 kv heads, 12 us, one run after the other 31.
+        // (Three may be long: 8 prompts of ~100 behind 40 11.7 us, by waves 17.4.)
+        append_keys(p, h, t, n, blk, off);
+        append_values(p, h, t, n, blk, off);
+      }
+    });
     return;
   }
   append_q(p, b - run_blocks);
