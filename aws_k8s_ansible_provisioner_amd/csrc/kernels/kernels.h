@@ -151,7 +151,8 @@ struct ScaledAttn {
   float eps;
 };
 void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s);
-void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, hipStream_t s);
+// waves: 8, or 4 (a tile of 256 rows is then two workgroups')
+void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, int waves, hipStream_t s);
 
 // ---- gemm.hip ----
 int gemm_splitk_choice(int M, int N, int K);

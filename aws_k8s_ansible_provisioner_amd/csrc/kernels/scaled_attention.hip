@@ -455,22 +455,24 @@ __device__ __forceinline__ float half_sum(float x) {
 __device__ __forceinline__ int row_key(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
 
 constexpr int kKeys = 64;
-constexpr int kSplitTiles = 8;     // key tiles that a part of a split tile takes at least
+// Key tiles that a part of a split tile takes at least: 700 tokens behind 300 (16 / 8 heads) 28 us, with 8 36.5; 1500 of
+// one kv head of 8 29 and 37.
+constexpr int kSplitTiles = 4;
 
 // key tiles of a tile's rows, and the parts that they are cut into
 struct Tile {
   int seq, row0, q0, q_len, ctx, keys, ntiles, parts;
 };
 template <int ROWS>
-__device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int tile) {
+__device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int seq, int row0) {
   Tile t;
-  t.seq = __builtin_amdgcn_readfirstlane(p.tile_seq[tile]);
-  t.row0 = __builtin_amdgcn_readfirstlane(p.tile_row[tile]);
-  t.q0 = p.q_start[t.seq];
-  t.q_len = p.q_start[t.seq + 1] - t.q0;
-  t.ctx = p.seq_lens[t.seq] - t.q_len;
-  t.keys = keys_of(p, t.seq);
-  const int last = min(t.q_len - 1, (t.row0 + ROWS - 1) / p.G);
+  t.seq = seq;
+  t.row0 = row0;
+  t.q0 = p.q_start[seq];
+  t.q_len = p.q_start[seq + 1] - t.q0;
+  t.ctx = p.seq_lens[seq] - t.q_len;
+  t.keys = keys_of(p, seq);
+  const int last = row0 >= t.q_len * p.G ? -1 : min(t.q_len - 1, (row0 + ROWS - 1) / p.G);
   t.ntiles = last < 0 ? 0 : max(0, min(t.ctx + last, t.keys - 1)) / kKeys + 1;
   t.parts = max(1, min(p.num_parts, t.ntiles / kSplitTiles));
   return t;
@@ -481,14 +483,17 @@ __device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int tile) {
 // next ones asked for) and the weights of the next tile.  Of eight waves the later four go half a step behind: the two
 // waves of a SIMD are in different halves, one's products beside the other's exponentials.
 template <int NW>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p) {
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p, int subs) {
   constexpr bool LATE = NW == 8;
   constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
   __shared__ __attribute__((aligned(16))) bf16 lds[2][2][kKeys * D];    // [K | V][buffer]
   const int flat = gridDim.x - 1 - blockIdx.x;     // the map rises by work: longest tiles first
   const int item = __builtin_amdgcn_readfirstlane(flat / p.Hkv), kvh = flat - item * p.Hkv;
   const int tile = __builtin_amdgcn_readfirstlane(item / p.num_parts), part = item - tile * p.num_parts;
-  const Tile T = tile_of<ROWS>(p, tile);
+  const int named = __builtin_amdgcn_readfirstlane(tile / subs);      // the map's tile, which subs workgroups share
+  const int seq = __builtin_amdgcn_readfirstlane(p.tile_seq[named]);
+  const int first_row = __builtin_amdgcn_readfirstlane(p.tile_row[named]) + (tile - named * subs) * ROWS;
+  const Tile T = tile_of<ROWS>(p, seq, first_row);
   if (part >= T.parts || T.ntiles == 0) return;
   const int ta = __builtin_amdgcn_readfirstlane(T.ntiles * part / T.parts);
   const int tb = __builtin_amdgcn_readfirstlane(T.ntiles * (part + 1) / T.parts);
@@ -764,10 +769,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
 
 // The parts of split tiles: 32 threads to a row, 8 rows to a workgroup.
 template <int ROWS>
-__global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p) {
+__global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p, int subs) {
   const int item = blockIdx.x / (ROWS / 8), sub = blockIdx.x - item * (ROWS / 8);
-  const int tile = item / p.Hkv, kvh = item - tile * p.Hkv;
-  const Tile T = tile_of<ROWS>(p, tile);
+  const int tile = item / p.Hkv, kvh = item - tile * p.Hkv, named = tile / subs;
+  const Tile T = tile_of<ROWS>(p, p.tile_seq[named], p.tile_row[named] + (tile - named * subs) * ROWS);
   if (T.parts <= 1) return;
   const int row = sub * 8 + (threadIdx.x >> 5), d0 = (threadIdx.x & 31) * 4;
   const int R = T.row0 + row, pos = R / p.G;
@@ -809,15 +814,17 @@ void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
     scaled_merge_kernel<<<dim3(num_seqs, p.Hkv), 256, merging * sizeof(float), s>>>(q);
 }
 
-void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, hipStream_t s) {
+void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, int waves, hipStream_t s) {
   if (num_tiles == 0) return;
-  const int grid = num_tiles * p.Hkv * p.num_parts;
-  if (tile_rows == 256) scaled_prefill_kernel<8><<<grid, 512, 0, s>>>(p);
-  else scaled_prefill_kernel<4><<<grid, 256, 0, s>>>(p);
-  if (p.num_parts == 1) return;
-  const int merge = num_tiles * p.Hkv * (tile_rows / 8);
-  if (tile_rows == 256) scaled_prefill_merge_kernel<256><<<merge, 256, 0, s>>>(p);
-  else scaled_prefill_merge_kernel<128><<<merge, 256, 0, s>>>(p);
+  const int subs = tile_rows / (32 * waves), tiles = num_tiles * subs, grid = tiles * p.Hkv * p.num_parts;
+  const int merge = tiles * p.Hkv * (4 * waves);
+  if (waves == 8) {
+    scaled_prefill_kernel<8><<<grid, 512, 0, s>>>(p, subs);
+    if (p.num_parts > 1) scaled_prefill_merge_kernel<256><<<merge, 256, 0, s>>>(p, subs);
+  } else {
+    scaled_prefill_kernel<4><<<grid, 256, 0, s>>>(p, subs);
+    if (p.num_parts > 1) scaled_prefill_merge_kernel<128><<<merge, 256, 0, s>>>(p, subs);
+  }
 }
 
 }  // namespace akap

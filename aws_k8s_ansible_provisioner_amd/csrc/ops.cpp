@@ -552,7 +552,8 @@ void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional
                               Tensor v_cache, Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start,
                               Tensor tile_seq, Tensor tile_row, std::optional<Tensor> positions,
                               std::optional<Tensor> cos_sin, std::optional<Tensor> q_w, int64_t G, double scale,
-                              double eps, int64_t tile_rows, int64_t parts, std::optional<Tensor> part) {
+                              double eps, int64_t tile_rows, int64_t waves, int64_t parts,
+                              std::optional<Tensor> part) {
   auto p = scaled_params(out, k_cache, v_cache, scales, block_tables, seq_lens, G, scale);
   TORCH_CHECK(tile_rows == 128 || tile_rows == 256, "tile_rows must be 128 or 256");
   const int64_t B = seq_lens.numel();
@@ -560,7 +561,8 @@ void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional
     TORCH_CHECK(t->scalar_type() == at::kInt && t->is_contiguous(), "q_start / tile maps must be contiguous int32");
   TORCH_CHECK(q_start.numel() >= B + 1 && tile_row.numel() >= tile_seq.numel(), "q_start / tile maps too short");
   check_same_device(out, {&q_start, &tile_seq, &tile_row});
-  TORCH_CHECK(parts > 0 && tile_seq.numel() * p.Hkv * std::max<int64_t>(parts, 32) < (1LL << 31) &&
+  TORCH_CHECK(waves == 4 || (waves == 8 && tile_rows == 256), "waves must be 4, or 8 with tiles of 256 rows");
+  TORCH_CHECK(parts > 0 && tile_seq.numel() * 2 * p.Hkv * std::max<int64_t>(parts, 32) < (1LL << 31) &&
                   out.size(0) * G < (1LL << 31),
               "too many rows");
   // split tiles: per (tile, part, kv head) and row 128 sums, then all rows' maxima, then all rows' sums
@@ -598,7 +600,7 @@ void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional
   p.tile_seq = tile_seq.data_ptr<int>();
   p.tile_row = tile_row.data_ptr<int>();
   const c10::DeviceGuard g(out.device());
-  akap::launch_scaled_prefill(p, tile_seq.numel(), (int)tile_rows, cur_stream());
+  akap::launch_scaled_prefill(p, tile_seq.numel(), (int)tile_rows, (int)waves, cur_stream());
 }
 
 void l2_prefetch(std::vector<Tensor> ts, Tensor sink) {
@@ -1631,7 +1633,7 @@ TORCH_LIBRARY(akap, m) {
       "scaled_attention_prefill(Tensor(a!) out, Tensor? q, Tensor? qkv, Tensor k_cache, Tensor v_cache, "
       "Tensor scales, Tensor block_tables, Tensor seq_lens, Tensor q_start, Tensor tile_seq, Tensor tile_row, "
       "Tensor? positions, Tensor? cos_sin, Tensor? q_w, int G, float scale, float eps, int tile_rows=128, "
-      "int parts=1, Tensor(b!)? part=None) -> ()");
+      "int waves=4, int parts=1, Tensor(b!)? part=None) -> ()");
   m.def(
       "sample(Tensor logits, Tensor temperature, Tensor top_k, Tensor top_p, Tensor seeds, "
       "Tensor steps, Tensor(a!) out_tokens, Tensor(b!) out_logprobs, "

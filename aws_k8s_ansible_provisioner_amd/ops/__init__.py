@@ -441,10 +441,16 @@ def scaled_attention_decode_fused(out, qkv, k_cache, v_cache, scales, block_tabl
                                    workspace, num_parts, part_size)
 
 
-def scaled_prefill_parts(grid: int, tile_rows: int, max_len: int) -> int:
-    """Parts along the keys that prompt tiles are cut into: as many as fill the card with one workgroup of
-    eight waves (tile_rows 256) or two of four to a CU, each of 512 keys or more."""
-    return max(1, min((512 if tile_rows == 128 else 256) // max(grid, 1), max_len // 512, 16))
+def scaled_prefill_plan(tiles: int, tile_rows: int, max_len: int) -> tuple[int, int]:
+    """(waves of a workgroup, parts along the keys) for prompt tiles, times kv heads, of sequences of at most
+    max_len keys.  Eight waves take a tile of 256 rows whole; where sequences are short, or the tiles few and the
+    keys not many, two workgroups of four do better: 24 prompts of ~250 (32 / 4 heads) 68 us, with eight waves 72,
+    4 of ~400 (16 / 8) 20.8 and 23.3, 700 tokens behind 300 27.8 and 30.7; but 2 of 1500 (32 / 8) 60 and 54, 8 of
+    2048 356 and 327, 1000 behind 9000 (16 / 8) 111 and 98.  Parts: as many as fill the card, one workgroup of eight
+    waves or two of four to a CU, of 512 keys or more as far as the host knows."""
+    waves = 8 if tile_rows == 256 and max_len > 512 and not (tiles < 128 and max_len <= 4096) else 4
+    grid = tiles * tile_rows // (32 * waves)
+    return waves, max(1, min((256 if waves == 8 else 512) // max(grid, 1), max_len // 512, 16))
 
 
 def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start, tile_seq,
@@ -458,8 +464,9 @@ def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq
     max_len: the longest sequence's keys where the host knows them (else what the block tables hold); a map of
     few tiles over many keys is cut along the keys, by scratch of 520 bytes per row and part."""
     if _native(out):
-        parts = scaled_prefill_parts(tile_seq.numel() * k_cache.shape[1], tile_rows,
-                                     block_tables.shape[1] * k_cache.shape[2] if max_len is None else max_len)
+        waves, parts = scaled_prefill_plan(tile_seq.numel() * k_cache.shape[1], tile_rows,
+                                           block_tables.shape[1] * k_cache.shape[2] if max_len is None
+                                           else max_len)
         part = None
         if parts > 1:
             part = torch.empty(tile_seq.numel() * k_cache.shape[1] * parts * tile_rows * 130,
@@ -468,7 +475,7 @@ def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq
         torch.ops.akap.scaled_attention_prefill(out, None if qprep is not None else q, qkv, k_cache, v_cache,
                                                 scales, block_tables, seq_lens, q_start, tile_seq, tile_row,
                                                 positions, cos_sin, q_w, gqa_group, scale, eps, tile_rows,
-                                                parts, part)
+                                                waves, parts, part)
         return out
     _check_scaled_attention(out, k_cache, v_cache, scales, block_tables, seq_lens, gqa_group, scale)
     if tile_rows not in (64, 128, 256):
