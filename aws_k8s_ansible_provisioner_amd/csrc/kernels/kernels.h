@@ -149,6 +149,7 @@ struct ScaledAttn {
   const __bf16* q_w;
   const __bf16* k_w;
   float eps;
+  int new_key;               // fused decode: where in LDS (set by the launcher)
 };
 void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s);
 // waves: 8, or 4 (a tile of 256 rows is then two workgroups')

@@ -211,6 +211,9 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(ScaledAttn p) {
 struct NewRow {
   bf16x8 x, w;
   f32x4 c[2], s[2];
+  int64_t slot;    // -1: none
+  int page;
+  float was;       // the scale of the slot's page, of keys in the rows up to the key's, of values in the value's
 };
 __device__ __forceinline__ void new_row_load(NewRow& n, const ScaledAttn& p, int seq, int kvh) {
   const int G = p.G, row = min((int)threadIdx.x >> 4, G + 1), j = threadIdx.x & 15;
@@ -218,9 +221,13 @@ __device__ __forceinline__ void new_row_load(NewRow& n, const ScaledAttn& p, int
   n.x = *reinterpret_cast<const bf16x8*>(p.qkv + (size_t)seq * p.qkv_stride + head * D + 8 * j);
   const bf16* w = row < G ? p.q_w : row == G ? p.k_w : nullptr;
   n.w = w != nullptr ? *reinterpret_cast<const bf16x8*>(w + 8 * j) : bf16x8{};
-  const int64_t pos = p.positions[seq];
+  const int64_t pos = p.positions[seq], slot = p.slots[seq];
   const f32x4* cs = reinterpret_cast<const f32x4*>(
       p.cos_sin + (size_t)(pos < 0 ? 0 : pos < p.max_pos ? pos : p.max_pos - 1) * D + 8 * (j & 7));
+  n.slot = slot < (int64_t)p.num_blocks * p.BS ? slot : -1;
+  const int64_t page = n.slot < 0 ? 0 : (int64_t)p.num_blocks * p.BS < (1ll << 31) ? (uint32_t)n.slot / (uint32_t)p.BS : n.slot / p.BS;
+  n.page = (int)page;
+  n.was = (row > G ? p.v_scale : p.k_scale)[page * p.Hkv + kvh];
   n.c[0] = cs[0];
   n.c[1] = cs[1];
   n.s[0] = cs[16];
@@ -232,10 +239,15 @@ __device__ __forceinline__ float row16_max(float v) {
   v = fmaxf(v, dpp_mov<0x141>(v));
   return fmaxf(v, dpp_mov<0x140>(v));
 }
-// q to LDS; where the partition holds the row's last key, the new key and value into their page, whose scales (or
-// -1: no slot) go to LDS too.  As the append kernel does it, by 16 threads.
-__device__ __forceinline__ void new_row_put(NewRow& n, const ScaledAttn& p, int seq, int kvh, bool writes, bf16* q_s,
-                                            float* scale_s) {
+// What the workgroup that holds the row's last key keeps of it in LDS: the codes (for the chunk that has it: nobody waits
+// for what is stored), the page's scales (of no slot -1), and whether its other codes were rounded anew.
+struct NewKey {
+  uint8_t k[D], v[D];
+  float scale[2];
+  int grown[2];
+};
+// q to LDS; `writes`: the new key and value into their page, as the append kernel does it, by 16 threads.
+__device__ __forceinline__ void new_row_put(NewRow& n, const ScaledAttn& p, int kvh, bool writes, bf16* q_s, NewKey* key) {
   const int G = p.G, row = threadIdx.x >> 4, j = threadIdx.x & 15;
   if (row >= G + 2) return;
   float x[8];
@@ -250,30 +262,74 @@ __device__ __forceinline__ void new_row_put(NewRow& n, const ScaledAttn& p, int 
     return;
   }
   if (!writes) return;
-  const bool value = row > G;
-  const int64_t slot = p.slots[seq];
-  if (slot < 0 || slot >= (int64_t)p.num_blocks * p.BS) {
-    if (j == 0) scale_s[value] = -1.f;
+  const int value = row > G;
+  if (n.slot < 0) {
+    if (j == 0) {
+      key->scale[value] = -1.f;
+      key->grown[value] = 0;
+    }
     return;
   }
-  const int64_t at = slot / p.BS * p.Hkv + kvh;
-  const int off = (int)(slot % p.BS);
+  const int64_t at = (int64_t)n.page * p.Hkv + kvh;
+  const int off = (int)(n.slot - (int64_t)n.page * p.BS);
   uint8_t* codes = (value ? p.v_cache : p.k_cache) + at * p.BS * D;
-  float* scale = (value ? p.v_scale : p.k_scale) + at;
   float most = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) most = fmaxf(most, scale_mag(x[e]));
-  const int exp = page_exp<16>(row16_max(most), scale, codes, off, p.BS);
+  const int need = scale_exp(row16_max(most)), was = off > 0 ? stored_exp(n.was) : -100, exp = max(need, was);
+  const bool grown = off > 0 && need > was;
+  if (grown) {
+    codes_grow<16>(codes, was - need, p.BS);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
   const float inv = exp_scale(-exp);
-  const uint32_t lo = codes4(x[0], x[1], x[2], x[3], inv), hi = codes4(x[4], x[5], x[6], x[7], inv);
+  const u32x2 c = {codes4(x[0], x[1], x[2], x[3], inv), codes4(x[4], x[5], x[6], x[7], inv)};
+  *reinterpret_cast<u32x2*>((value ? key->v : key->k) + 8 * j) = c;
   if (!value) {
-    *reinterpret_cast<u32x2*>(codes + k_swz_offset(off) + k_dim_offset(8 * j)) = u32x2{lo, hi};
+    *reinterpret_cast<u32x2*>(codes + k_swz_offset(off) + k_dim_offset(8 * j)) = c;
   } else {
     uint8_t* to = codes + (size_t)(off >> 3) * D * 8 + 64 * j + (off & 7);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) to[8 * e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+    for (int e = 0; e < 8; ++e) to[8 * e] = (uint8_t)(c[e >> 2] >> (8 * (e & 3)));
   }
-  if (j == 0) scale_s[value] = exp_scale(exp);
+  if (j == 0) {
+    (value ? p.v_scale : p.k_scale)[at] = exp_scale(exp);
+    key->scale[value] = exp_scale(exp);
+    key->grown[value] = grown;
+  }
+  if (grown) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+// the new key into its chunk's registers: token `tok` of the 32
+__device__ __forceinline__ void put_k(Chunk& c, const NewKey* key, int tok) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const bool mine = (lane & 15) == ((tok >> 3) << 2 | (tok & 3));
+  const bool upper = (tok >> 2) & 1;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(key->k + 64 * i + 16 * g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      c.k[0][i][e] = mine && !upper ? x[e] : c.k[0][i][e];
+      c.k[1][i][e] = mine && upper ? x[e] : c.k[1][i][e];
+    }
+  }
+}
+__device__ __forceinline__ void put_v(Chunk& c, const NewKey* key, int tok) {
+  const int lane = threadIdx.x & 63, r = lane & 15;
+  const bool mine = (lane >> 4) == tok >> 3, upper = tok & 4;
+  const int at = 8 * (tok & 3);
+  const uint32_t keep = ~(0xffu << at);
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const uint32_t x = *reinterpret_cast<const uint16_t*>(key->v + 32 * n + 2 * r);
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const uint32_t b = ((x >> (8 * d)) & 0xff) << at;
+      const uint32_t lo = c.v[n][2 * d], hi = c.v[n][2 * d + 1];
+      c.v[n][2 * d] = mine && !upper ? (lo & keep) | b : lo;
+      c.v[n][2 * d + 1] = mine && upper ? (hi & keep) | b : hi;
+    }
+  }
 }
 
 template <bool FUSED>
@@ -312,32 +368,33 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   load_k(c, rsrc_of(p.k_cache, 0));
   load_v(c, rsrc_of(p.v_cache, 0));
   bf16x8 q[4];
+  NewKey* key = nullptr;             // where the row's last key is new and this partition's
   if constexpr (FUSED) {
     bf16* q_s = reinterpret_cast<bf16*>(lds);            // [G][D]
-    float* scale_s = lds + G * D / 2;                    // the new entries' scales
+    key = reinterpret_cast<NewKey*>(lds + p.new_key);
     const bool writes = keys > 0 && part == nparts - 1;
-    new_row_put(fresh, p, seq, kvh, writes, q_s, scale_s);
-    if (writes) {
-      // what was written is read again by the chunks of its page: whole pages lie in a partition
-      __syncthreads();
+    new_row_put(fresh, p, kvh, writes, q_s, key);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // LDS alone: the first chunk stays on its way
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (!writes || key->scale[0] < 0.f) key = nullptr;
+    if (key != nullptr) {
       const int last = (keys - 1) / BS;
-      if (column == last && scale_s[0] >= 0.f) {
-        ks = scale_s[0] * p.scale_log2;
-        vs = scale_s[1];
+      if (column == last) {
+        ks = key->scale[0] * p.scale_log2;
+        vs = key->scale[1];
       }
-      if (t0 < end && t0 / BS == last) {
+      // a page rounded anew lies in this partition whole: what was read of it before is read again
+      if ((key->grown[0] | key->grown[1]) != 0 && t0 < end && t0 / BS == last) {
         load_k(c, rsrc_of(p.k_cache, 0));
         load_v(c, rsrc_of(p.v_cache, 0));
       }
-    } else {                                             // the first chunk stays on its way
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       q[i] = *reinterpret_cast<const bf16x8*>(q_s + min(r, G - 1) * D + 16 * g + 64 * (i >> 1) + 8 * (i & 1));
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();                        // (the rows' sums go where q and the scales are)
+    __builtin_amdgcn_s_barrier();                        // (the rows' sums go where q is)
   } else {
     const bf16* qp = p.q + ((size_t)q_tok * p.Hq + kvh * G + min(r, G - 1)) * D + 16 * g;
 #pragma unroll
@@ -353,8 +410,11 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   for (int t = t0, i = 0; t < end; t += 128, ++i) {
     const bool some = page_of(i) >= 0;
     float x[8];
+    const bool has = FUSED && key != nullptr && (uint32_t)(keys - 1 - t) < 32;
+    if (has) put_k(c, key, keys - 1 - t);
     if (some) chunk_scores(x, q, c, lane_f(ks, i));
     load_k(c, rsrc_of(p.k_cache, i + 1));
+    if (has) put_v(c, key, keys - 1 - t);
     if (some) chunk_rows(st, x, c, lane_f(vs, i), end - t);
     load_v(c, rsrc_of(p.v_cache, i + 1));
   }
@@ -798,15 +858,22 @@ __global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p,
 
 void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
   if (num_seqs == 0) return;
-  // Coarser partitions than asked for, in whole ones: under 512 keys a wave has too few chunks to pay for the merge,
-  // and more than 64 of them cost it more than they give.
+  // Coarser partitions than asked for, in whole ones.  One for up to 512 keys (1 row at 333, 16 / 8 heads, 5.5 us, in two
+  // 7.1), at most 64 (3 rows at ~25000, 8 / 1 heads, 16.2 us, in 118 20.5), else 256 keys or more (1 row at 4000 8.7 us,
+  // 512 10.8); and rows that fill the card by themselves need none, up to 2048 keys (beyond, a long row among short ones
+  // would hold up the step): 64 rows at ~1500 keys of 32 / 8 heads in partitions of 512, 1024, 2048 44, 42, 36 us, 128
+  // at ~1050 65, 60, 53, 16 at ~2250 in 256, 768, 1536 20.6, 18, 22.
   ScaledAttn q = p;
-  const int by = std::min(std::max((511 + p.part_size) / p.part_size, (p.num_parts + 63) / 64),
+  const int64_t rows = (int64_t)num_seqs * p.Hkv;
+  const int fill = (int)std::min<int64_t>((p.num_parts * rows + 511) / 512, (2047 + p.part_size) / p.part_size);
+  const int by = std::min(std::max({((p.num_parts * p.part_size <= 512 ? 511 : 255) + p.part_size) / p.part_size, (p.num_parts + 63) / 64, fill}),
                           kDecodeMaxPart / p.part_size);
   q.part_size = p.part_size * by;
   q.num_parts = (p.num_parts + by - 1) / by;
   const size_t merging = q.num_parts > 1 ? 16 * (D + 4) : 0;
-  const size_t smem = std::max<size_t>(4 * p.G * (D + 4) + 8 * p.G, merging) * sizeof(float);
+  const size_t rows_s = std::max<size_t>(4 * p.G * (D + 4) + 8 * p.G, merging);
+  q.new_key = (int)(rows_s + 3) / 4 * 4;
+  const size_t smem = p.qkv != nullptr ? q.new_key * sizeof(float) + sizeof(NewKey) : rows_s * sizeof(float);
   const dim3 grid(num_seqs, p.Hkv, q.num_parts);
   if (p.qkv != nullptr) scaled_decode_kernel<true><<<grid, 256, smem, s>>>(q);
   else scaled_decode_kernel<false><<<grid, 256, smem, s>>>(q);
