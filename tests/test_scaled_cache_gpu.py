@@ -43,10 +43,15 @@ def run_append(case, H, G, slots, decode=False, num_decode=0, q_rows=-1, rope=Tr
     (8, 4, 128, 9, list(range(130, 500)) + [1000], True),                # pages longer than a wave's rows
     (5, 1, 32, 3, [], True),
     (0, 2, 32, 4, [31, 32, 33], False),                                  # no query heads
+    (2, 2, 32, 60, [32 * i + i % 29 + j for i in range(50) for j in range(3)], True),   # many short runs
+    (2, 1, 32, 12, list(range(20, 43)) + list(range(90, 101)) + list(range(128, 130)), True),   # three in a span
+    (2, 2, 64, 9, list(range(7, 64)) + list(range(130, 192)) + list(range(320, 384)), False),
+    (1, 1, 256, 4, list(range(300, 700)), True),
 ])
 def test_append(H, G, page, pages, slots, norm):
     case = make(21, H, G, len(slots), slots, page, pages, norm, std=3.0)
     qkv, k, v, s, pos, sl, cs, w = case
+    ops.check_scaled_slots(sl, page)
     for decode in (False, True):
         k1, v1, s1, q = run_append(case, H, G, slots, decode)
         check_append(qkv, k, v, s, pos, sl, cs, w, H, G, k1, v1, s1, q if H and slots else None)
@@ -124,6 +129,11 @@ def want_rows(c, lens, scale=0.1):
     (5, 1, 96, [97, 400, 0, 383, 384, 385], 2, 384),
     (8, 8, 32, [700, 1], 3, 256),
     (12, 4, 32, [0, 0], 2, 128),
+    (16, 1, 32, [2100, 3, 1025], 9, 256),                 # merges of one, two, .. groups of threads
+    (3, 1, 32, [2100, 3, 1025], 9, 256),
+    (2, 2, 32, [3000, 513], 24, 128),
+    (16, 2, 32, [700, 40] * 140, 6, 128),                 # rows that fill the card
+    (4, 4, 64, [9000], 128, 128),
 ])
 def test_decode(H, G, page, lens, parts, size):
     c = attention_case(31, H, G, page, lens, [1] * len(lens))
@@ -177,17 +187,29 @@ def test_decode_extreme_scores():
 
 
 # ------------------------------------------------------------------------------------------------ prompts
-def run_prompt(c, lens, new, H, G, rows, scale=0.1):
+def run_prompt(c, lens, new, H, G, rows, scale=0.1, max_len=None):
     q, k, v, s, t, n, start = gpu(*c)
     out = torch.full_like(q, 9.0)
     st = torch.tensor(start, dtype=torch.int32, device=DEV)
     ops.scaled_attention_prefill(out, q, k, v, s, t, n, st, *tiles(lens, new, H // G, rows), H // G, scale,
-                                 tile_rows=rows)
+                                 tile_rows=rows, max_len=max_len)
     torch.cuda.synchronize()
     return out
 
 
-@pytest.mark.parametrize("rows", [128, 256])
+# (rows of a tile, the bound on the keys that the host states: it alone chooses waves and parts)
+FORMS = [(128, None), (128, 100000), (256, None), (256, 2000), (256, 100000)]
+
+
+def test_prompt_forms():
+    """What FORMS stand for, for few tiles."""
+    assert [ops.scaled_prefill_plan(4, r, n) for r, n in ((128, 500), (128, 100000), (256, 500), (256, 2000),
+                                                          (256, 100000))] == \
+        [(4, 1), (4, 16), (4, 1), (4, 3), (8, 16)]
+    assert ops.scaled_prefill_plan(4096, 256, 2048) == (8, 1) and ops.scaled_prefill_plan(64, 256, 10016) == (8, 4)
+
+
+@pytest.mark.parametrize("rows,max_len", FORMS)
 @pytest.mark.parametrize("H,G,page,lens,new", [
     (1, 1, 32, [1], [1]),
     (4, 2, 32, [63, 64, 65, 1], [63, 64, 65, 1]),
@@ -195,14 +217,25 @@ def run_prompt(c, lens, new, H, G, rows, scale=0.1):
     (5, 1, 96, [200, 97], [130, 97]),
     (8, 8, 32, [700], [260]),
     (20, 1, 32, [50, 2000], [50, 9]),
+    (2, 1, 32, [2500, 1100, 257], [3, 200, 257]),
+    (3, 1, 64, [511, 512, 513, 0], [2, 512, 1, 0]),
 ])
-def test_prompts(H, G, page, lens, new, rows):
+def test_prompts(H, G, page, lens, new, rows, max_len):
     c = attention_case(41, H, G, page, lens, new)
-    close(run_prompt(c, lens, new, H, G, rows), *want_rows(c, lens))
+    close(run_prompt(c, lens, new, H, G, rows, max_len=max_len), *want_rows(c, lens))
 
 
-@pytest.mark.parametrize("rows", [128, 256])
-def test_prompts_beside_codes_that_are_no_numbers(rows):
+def test_prompts_extreme_scores():
+    """Scores of some thousands, rising along the keys: every tile moves the maximum."""
+    lens, new = [700], [300]
+    c = attention_case(45, 2, 1, 32, lens, new)
+    c = (c[0] * 40, *c[1:])
+    for rows, max_len in FORMS:
+        close(run_prompt(c, lens, new, 2, 1, rows, 2.0, max_len), *want_rows(c, lens, 2.0))
+
+
+@pytest.mark.parametrize("rows,max_len", FORMS)
+def test_prompts_beside_codes_that_are_no_numbers(rows, max_len):
     lens, new = [45, 330], [45, 70]
     c = attention_case(42, 4, 2, 32, lens, new)
     want = want_rows(c, lens)
@@ -212,15 +245,26 @@ def test_prompts_beside_codes_that_are_no_numbers(rows):
         blk = int(t[b, m // 32])
         k.view(-1, 2, 32 * D)[blk][:, ki[m % 32:].reshape(-1)] = 0x7f
         v.view(-1, 2, 32 * D)[blk][:, vi[m % 32:].reshape(-1)] = 0xff
-    close(run_prompt(c, lens, new, 4, 2, rows), *want)
+    close(run_prompt(c, lens, new, 4, 2, rows, max_len=max_len), *want)
 
 
-@pytest.mark.parametrize("rows", [128, 256])
-def test_prompts_pages_outside_the_cache(rows):
+@pytest.mark.parametrize("rows,max_len", FORMS)
+def test_prompts_pages_outside_the_cache(rows, max_len):
     lens, new = [200, 33], [150, 33]
     c = attention_case(43, 4, 2, 32, lens, new, bad={(0, 0): -1, (0, 3): 1 << 29, (0, 6): -5, (1, 0): 77777})
-    out = run_prompt(c, lens, new, 4, 2, rows)
+    out = run_prompt(c, lens, new, 4, 2, rows, max_len=max_len)
     close(out, *want_rows(c, lens))
+
+
+@pytest.mark.parametrize("rows,max_len", FORMS)
+def test_prompts_of_no_visible_keys(rows, max_len):
+    """All pages outside the cache, or no length at all: rows of zeros."""
+    lens, new = [300, 40], [100, 40]
+    c = attention_case(46, 4, 2, 32, lens, new, bad={(0, i): -1 for i in range(10)})
+    q, k, v, s, t, n, start = c
+    n = torch.tensor([300, 0], dtype=torch.int32)
+    out = run_prompt((q, k, v, s, t, n, start), [300, 40], new, 4, 2, rows, max_len=max_len)
+    assert not out.any()
 
 
 def test_prompts_leave_other_rows():
@@ -256,6 +300,8 @@ def step_case(seed, H, G, page, past, norm, room=0):
     (4, 1, 64, [0, 63, 64, 127, 128, 500], False, 4, 128),
     (14, 1, 32, [700, 5], True, 3, 256),
     (5, 1, 96, [383, 384, 10], True, 2, 384),
+    (4, 2, 256, [700, 255, 256, 300, 513], False, 4, 256),
+    (15, 1, 32, [40, 64], True, 1, 128),                  # more query heads than one launch takes
 ])
 def test_fused_step(H, G, page, past, norm, parts, size):
     lens, qkv, k, v, s, t, n, pos, sl, cs, w = step_case(51, H, G, page, past, norm)
@@ -276,6 +322,62 @@ def test_fused_step(H, G, page, past, norm, parts, size):
     close(out, want, bound + q_bound(q, entries, t, lens, start, 0.1))
 
 
+@pytest.mark.parametrize("page", [32, 64, 256])
+def test_fused_step_where_the_scale_grows(page):
+    """Every row's key and value are far louder than their page: its codes are rounded anew before they are read,
+    whichever chunk of the page a wave holds already."""
+    H, G = 4, 2
+    past = [1, 31, 33, 63, 65, 100, 127, 129, 191, 255]
+    lens, qkv, k, v, s, t, n, pos, sl, cs, w = step_case(55, H, G, page, past, False)
+    qkv[:, H * D:] *= 4096
+    k0, v0, s0 = k.clone(), v.clone(), s.clone()
+    k1, v1, s1 = gpu(k, v, s)
+    out = torch.empty(len(past), H, D, dtype=torch.bfloat16, device=DEV)
+    ops.scaled_attention_decode_fused(out, *gpu(qkv), k1, v1, s1, *gpu(t, n, pos, sl, cs, *w), H // G, 1e-5, 1e-6)
+    check_append(qkv, k0, v0, s0, pos, sl, cs, w, H, G, k1, v1, s1, None)
+    assert bool((s1.cpu()[:, sl // page] > s0[:, sl // page]).all())
+    q = orc.prepared(qkv, pos, cs, *w, H, G, 1e-6)[0]
+    entries = orc.codes(k1, v1) * s1.cpu().double()[..., None, None]
+    start = list(range(len(past) + 1))
+    want, bound = orc.attention(q, entries, t, lens, start, 1e-5)
+    close(out, want, bound + q_bound(q, entries, t, lens, start, 1e-5))
+
+
+def test_fused_step_of_padding():
+    """Rows without a slot append nothing, rows of no keys nothing either and are zero."""
+    H, G, page = 8, 2, 32
+    past = [40, 40, 40]
+    lens, qkv, k, v, s, t, n, pos, sl, cs, w = step_case(57, H, G, page, past, True)
+    sl = torch.tensor([-1, 10 ** 9, int(sl[2])])
+    n = torch.tensor([41, 41, 0], dtype=torch.int32)
+    k1, v1, s1 = gpu(k.clone(), v.clone(), s.clone())
+    out = torch.full((3, H, D), 5.0, dtype=torch.bfloat16, device=DEV)
+    for parts, size in ((1, 512), (3, 128)):
+        ws = ops.decode_workspace(3, G, H // G, parts, DEV)
+        ops.scaled_attention_decode_fused(out, *gpu(qkv), k1, v1, s1, *gpu(t, n, pos, sl, cs, *w), H // G, 0.1,
+                                          1e-6, workspace=ws, num_parts=parts, part_size=size)
+        torch.cuda.synchronize()
+        for a, b in ((k1, k), (v1, v), (s1, s)):
+            assert torch.equal(a.cpu(), b)
+        assert not out[2].any()
+        q = orc.prepared(qkv, pos, cs, *w, H, G, 1e-6)[0]
+        entries = orc.codes(k, v) * s.double()[..., None, None]
+        want, bound = orc.attention(q[:2], entries, t, [41, 41], [0, 1, 2], 0.1)
+        close(out[:2], want, bound + q_bound(q[:2], entries, t, [41, 41], [0, 1, 2], 0.1))
+
+
+def test_empty_batches():
+    q, k, v, s, t, n, start = gpu(*attention_case(58, 4, 2, 32, [40], [1]))
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    ops.scaled_attention_decode(q[:0], q[:0], k, v, s, t, n[:0], 2, 0.1)
+    ops.scaled_attention_prefill(q[:0], q[:0], k, v, s, t, n[:0], n[:1], none, none, 2, 0.1)
+    long = torch.empty(0, dtype=torch.int64, device=DEV)
+    ops.scaled_attention_decode_fused(q[:0], torch.empty(0, 8 * D, dtype=torch.bfloat16, device=DEV), k, v, s, t,
+                                      n[:0], long, long, ref.rope_cos_sin(16, D, 1e4).to(DEV), None, None, 2, 0.1,
+                                      1e-6)
+    torch.cuda.synchronize()
+
+
 def q_bound(q, entries, t, lens, start, scale):
     """What rounding q to bf16 (half a step, 2^-8) can change: each score by 2^-8 sum |q k| scale =: d, each
     weight by a factor between e^-2d and e^2d."""
@@ -294,9 +396,9 @@ def q_bound(q, entries, t, lens, start, scale):
     return off
 
 
-@pytest.mark.parametrize("rows", [128, 256])
+@pytest.mark.parametrize("rows,max_len", FORMS)
 @pytest.mark.parametrize("norm", [True, False])
-def test_prompt_step_prepares_its_queries(rows, norm):
+def test_prompt_step_prepares_its_queries(rows, max_len, norm):
     """A step of chunks: append without q, then the attention over the projection's rows."""
     H, G, page = 8, 2, 32
     lens, new = [90, 64, 3], [90, 20, 3]
@@ -315,7 +417,7 @@ def test_prompt_step_prepares_its_queries(rows, norm):
     ops.scaled_cache_append(x, out, k1, v1, s1, d[2], d[3], d[4], d[5], d[6], H, G, 1e-6, q_rows=0)
     st = torch.tensor(start, dtype=torch.int32, device=DEV)
     ops.scaled_attention_prefill(out, None, k1, v1, s1, d[0], d[1], st, *tiles(lens, new, H // G, rows), H // G, 0.1,
-                                 tile_rows=rows, qprep=(x, d[2], d[4], d[5], 1e-6))
+                                 tile_rows=rows, qprep=(x, d[2], d[4], d[5], 1e-6), max_len=max_len)
     torch.cuda.synchronize()
     check_append(qkv, k0, v0, s0, pos, sl, cs, w, H, G, k1, v1, s1, None)
     eq = orc.prepared(qkv, pos, cs, *w, H, G, 1e-6)[0]
