@@ -3,9 +3,9 @@
 //
 // A page's scale depends on all the entries that a call brings, and where it grows its old codes are rounded
 // anew, so a page and head belong to one workgroup, or a wave: the one that finds the page's first row of the call.
-// Rows whose slots follow each other inside a page are a run, its first row the leader; a workgroup looks over 32
-// rows of the batch for leaders (a wave over one, where rows are single tokens of their sequences) and takes each
-// run: magnitudes first, then the codes.  The caller keeps the rows of a page together, in rising slots.
+// Rows whose slots follow each other inside a page are a run, its first row the leader; a workgroup looks over a span
+// of 8 to 32 rows of the batch for leaders (a wave over one, where rows are single tokens of their sequences) and
+// takes each run: magnitudes first, then the codes.  The caller keeps the rows of a page together, in rising slots.
 #include "scaled_cache.h"
 #include "kernels.h"
 
@@ -231,11 +231,10 @@ __device__ __forceinline__ void append_run(const ScaledAppend& p, int h, int t, 
   }
 }
 
-// Rows [t0, t0 + ROWS) of the batch (ROWS <= 32): `run` for each run that begins there, the i-th of
-// count.  The slots of 64 rows, one to a
-// lane, tell where runs begin and, as a rule, end.
-template <int ROWS, typename F>
-__device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F& run) {
+// Rows [t0, t0 + rows) of the batch (rows <= 32): `run` for each run that begins there, the i-th, with whether the
+// runs are few and some of them long.  The slots of 64 rows, one to a lane, tell where runs begin and, as a rule, end.
+template <typename F>
+__device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, int rows, const F& run) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)p.num_blocks * p.BS;
   const bool narrow = cap < (1ll << 31);
@@ -248,8 +247,13 @@ __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F&
   const int off = (int)(mine - page * p.BS);
   const bool follows = mine >= 0 && before == mine - 1 && off != 0;
   const uint64_t on = __ballot(follows);
-  uint64_t leaders = __ballot(lane < ROWS && mine >= 0 && !follows);
+  uint64_t leaders = __ballot(lane < rows && mine >= 0 && !follows);
   const int count = __popcll(leaders);
+  uint64_t longer = on & on >> 1;
+  longer &= longer >> 2;
+  longer &= longer >> 4;
+  longer &= longer >> 8;            // 16 rows that each follow the one before
+  const bool few = count <= 3 && longer != 0;
   for (int i = 0; i < count; ++i) {
     const int l = __builtin_ctzll(leaders);
     leaders &= leaders - 1;
@@ -263,19 +267,20 @@ __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, const F&
       n += more == ~0ull ? 64 : __builtin_ctzll(~more);
       if (more != ~0ull) break;
     }
-    run(i, count, t0 + l, n, blk, o);
+    run(i, few, t0 + l, n, blk, o);
   }
 }
 
 template <int HELD>
-__global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int single_blocks, int run_blocks) {
+__global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int single_blocks, int run_blocks,
+                                                            int rows) {
   __shared__ float red[2][4];
   int b = blockIdx.x;
   if (b < single_blocks) {
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = 2 * p.Hkv;
     const int item = b * 4 + w, t = item / per, h = (item - t * per) >> 1;
     if (t >= p.singles) return;
-    for_runs<1>(p, t, [&](int, int, int t, int n, int64_t blk, int off) {
+    for_runs(p, t, 1, [&](int, bool, int t, int n, int64_t blk, int off) {
       if (item & 1) append_values(p, h, t, n, blk, off);
       else append_keys(p, h, t, n, blk, off);
     });
@@ -285,15 +290,17 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
   if (b < run_blocks) {
     const int span = b / p.Hkv, h = b - span * p.Hkv;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for_runs<32>(p, p.singles + 32 * span, [&](int i, int count, int t, int n, int64_t blk, int off) {
-      if (count <= 3) {
+    for_runs(p, p.singles + rows * span, rows, [&](int i, bool few, int t, int n, int64_t blk, int off) {
+      if (few) {
         append_run<HELD>(p, h, t, n, blk, off, red);
-      } else if ((i & 3) == w) {
-        // Many short runs, a wave to each: 64 sequences of 3 tokens, 8 kv heads, 12 us, one run after the other 31.
-        // (Three may be long: 8 prompts of ~100 behind 40 11.7 us, by waves 17.4.)
-        append_keys(p, h, t, n, blk, off);
-        append_values(p, h, t, n, blk, off);
+        return;
       }
+      // Many runs, or short ones: a wave to the keys or the values of each.  64 sequences of 3 tokens, 8 kv heads, in
+      // spans of 32 rows: 12 us, one run after the other 31; 3 of 2 tokens 5.4, else 10.4.  (Three may be long: 8
+      // prompts of ~100 behind 40 11.8 us, by waves 15.8.)
+      const int job = 2 * i + (i >> 1);
+      if ((job & 3) == w) append_keys(p, h, t, n, blk, off);
+      if ((job + 1 & 3) == w) append_values(p, h, t, n, blk, off);
     });
     return;
   }
@@ -305,12 +312,17 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
 void launch_scaled_append(const ScaledAppend& p, hipStream_t s) {
   const long per = 2 * p.Hkv;
   const long single = (p.singles * per + 3) / 4;
-  const long runs = (long)(p.T - p.singles + 31) / 32 * p.Hkv;
+  // Runs begin anywhere, and a span's are taken in turn: the smallest span of 8, 16 or 32 rows whose workgroups are
+  // at most 512, two to a unit.  8 kv heads, spans of 8, 16 and 32: 49 sequences of 3 tokens 8.2, 12.8 and 20.7 us; 8
+  // of ~130 10.0, 9.0 and 11.8; one of 1000 9.4, 7.7 and 6.9; 60 of ~200 46.4, 38.5 and 36.9.
+  int rows = 8;
+  while (rows < 32 && (long)(p.T - p.singles + rows - 1) / rows * p.Hkv > 512) rows *= 2;
+  const long runs = (long)(p.T - p.singles + rows - 1) / rows * p.Hkv;
   const long q = ((long)p.q_rows * ((p.Hq + kQHeads - 1) / kQHeads) + 15) / 16;
   if (single + runs + q == 0) return;
   const dim3 grid((unsigned)(single + runs + q));
-  if (p.BS <= 32) scaled_append_kernel<1><<<grid, 256, 0, s>>>(p, (int)single, (int)runs);
-  else scaled_append_kernel<2><<<grid, 256, 0, s>>>(p, (int)single, (int)runs);
+  if (p.BS <= 32) scaled_append_kernel<1><<<grid, 256, 0, s>>>(p, (int)single, (int)runs, rows);
+  else scaled_append_kernel<2><<<grid, 256, 0, s>>>(p, (int)single, (int)runs, rows);
 }
 
 }  // namespace akap
