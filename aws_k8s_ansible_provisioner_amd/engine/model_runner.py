@@ -457,7 +457,7 @@ class ModelRunner:
                           self.workspace, tile_rows=info.get("tile_rows") or self.tile_rows,
                           num_decode=nd,
                           v_tails=self.v_tails, tail_slot=v["tail_slot"],
-                          kv_scales=self.kv_scales)
+                          kv_scales=self.kv_scales, max_len=info.get("max_seq_len") or None)
         if self._ep_moe:
             moe_mod.ep_overflow_reset(self.device)
         h = self.model.forward(ids, batch, self.k_caches, self.v_caches)

@@ -57,6 +57,7 @@ class AttnBatch:
     tail_slot: Optional[torch.Tensor] = None
     # scaled 8-bit cache: per-layer scales [2, blocks, kv heads]; None = the other caches
     kv_scales: Optional[list] = None
+    max_len: Optional[int] = None  # longest sequence's keys (block tables are wider)
 
 
 @dataclasses.dataclass
@@ -396,7 +397,8 @@ class DecoderLM:
             ops.scaled_attention_prefill(
                 out, q, kc, vc, sc, batch.block_tables, batch.seq_lens, batch.q_start, batch.tile_seq,
                 batch.tile_row, G, self.scale, tile_rows=batch.tile_rows,
-                qprep=(qkv, batch.positions, self.cos_sin, lw.q_norm, self.cfg.rms_eps) if qp else None)
+                qprep=(qkv, batch.positions, self.cos_sin, lw.q_norm, self.cfg.rms_eps) if qp else None,
+                max_len=batch.max_len)
 
     def _attention(self, q, batch: AttnBatch, kc, vc, out, vt=None, qprep=None):
         if batch.is_prefill:

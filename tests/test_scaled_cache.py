@@ -234,6 +234,33 @@ def test_engine_on_a_scaled_cache():
         assert bool((s > 2.0 ** -100).any()) and bool((torch.frexp(s)[0] == 0.5).all())
 
 
+def test_engine_plans_prompts_by_their_longest_sequence(monkeypatch):
+    """Not by what the block tables could hold."""
+    from test_engine_cpu import _engine
+    from aws_k8s_ansible_provisioner_amd.engine.config import SamplingParams
+
+    seen, real = set(), ops.scaled_attention_prefill
+
+    def record(out, q, k, v, s, tables, lens, *a, max_len=None, **kw):
+        seen.add((int(lens.max()), max_len, tables.shape[1] * k.shape[2]))
+        return real(out, q, k, v, s, tables, lens, *a, max_len=max_len, **kw)
+
+    monkeypatch.setattr(ops, "scaled_attention_prefill", record)
+    eng = _engine("tiny-qwen3", kv_cache_dtype="fp8_scaled")
+    eng.generate(None, SamplingParams(max_tokens=2, temperature=0, ignore_eos=True),
+                 prompt_ids=[list(range(5, 45)), [7, 8, 9] * 14])
+    assert seen and all(longest == said < room for longest, said, room in seen)
+
+
+def test_prompt_plans():
+    for rows in (128, 256):
+        for tiles in (1, 7, 64, 500, 5000):
+            for n in (1, 500, 1000, 5000, 100000):
+                waves, parts = ops.scaled_prefill_plan(tiles, rows, n)
+                assert waves in (4, 8) and 32 * waves <= rows and 1 <= parts <= 16
+                assert parts == 1 or n >= 1024
+
+
 def test_engine_refuses_roles_and_blocks():
     from aws_k8s_ansible_provisioner_amd.engine.config import EngineConfig
 
