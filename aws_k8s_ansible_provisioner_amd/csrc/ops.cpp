@@ -332,9 +332,11 @@ static void check_scaled(const Tensor& k_cache, const Tensor& v_cache, const Ten
   CHECK_GPU(k_cache); CHECK_CONTIG(k_cache); CHECK_CONTIG(v_cache); CHECK_CONTIG(scales);
   TORCH_CHECK(k_cache.scalar_type() == at::kByte && v_cache.scalar_type() == at::kByte,
               "scaled cache: uint8 K and V (e4m3 codes)");
-  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(0) > 0 && k_cache.size(3) == 128,
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(0) > 0 && k_cache.size(1) > 0 && k_cache.size(1) < 65536 &&
+                  k_cache.size(3) == 128,
               "scaled cache: K [NB, Hkv, BS, 128]");
-  TORCH_CHECK(k_cache.size(2) > 0 && k_cache.size(2) % 32 == 0, "scaled cache: block size must be a multiple of 32");
+  TORCH_CHECK(k_cache.size(2) > 0 && k_cache.size(2) % 32 == 0 && k_cache.size(2) <= 65536,
+              "scaled cache: block size must be a multiple of 32, at most 65536");
   TORCH_CHECK(v_cache.dim() == 5 && v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) &&
                   v_cache.size(2) * 8 == k_cache.size(2) && v_cache.size(3) == 128 && v_cache.size(4) == 8,
               "scaled cache: V [NB, Hkv, BS/8, 128, 8]");
@@ -382,9 +384,12 @@ void scaled_cache_append(Tensor qkv, Tensor q_out, Tensor k_cache, Tensor v_cach
   TORCH_CHECK(Hq >= 0 && Hkv == k_cache.size(1), "scaled_cache_append: the cache has other kv heads");
   check_rows(qkv, Hq + 2 * Hkv);
   const int64_t T = qkv.size(0);
-  TORCH_CHECK(T < (1LL << 31) && singles >= 0 && singles <= T && q_rows >= -1 && q_rows <= T,
+  TORCH_CHECK(singles >= 0 && singles <= T && q_rows >= -1 && q_rows <= T,
               "scaled_cache_append: num_decode / q_rows out of range");
   if (q_rows < 0) q_rows = T;
+  // (a launch counts its threads in 32 bits)
+  TORCH_CHECK(T < (1LL << 30) && (singles / 2 + (T - singles) / 8 + 3) * Hkv + q_rows * ((Hq + 3) / 4) / 16 < (1LL << 24) - 1,
+              "scaled_cache_append: too many rows for a call");
   check_angles(qkv, positions, cos_sin, T);
   check_norm_weight(qkv, q_w);
   check_norm_weight(qkv, k_w);
@@ -470,7 +475,7 @@ static void set_parts(akap::ScaledAttn& p, const Tensor& out, int64_t B, int64_t
   TORCH_CHECK(num_parts > 0 && num_parts < 65536 && part_size > 0 && part_size % 128 == 0 &&
                   part_size <= akap::kDecodeMaxPart,
               "part_size must be a multiple of 128, at most ", akap::kDecodeMaxPart);
-  TORCH_CHECK(B < (1LL << 31) && p.Hkv < 65536, "too many rows");
+  TORCH_CHECK(B < (1LL << 24) && B * p.Hkv < (1LL << 31), "too many rows for a call");
   p.num_parts = num_parts;
   p.part_size = part_size;
   if (num_parts == 1) return;
@@ -562,9 +567,10 @@ void scaled_attention_prefill(Tensor out, std::optional<Tensor> q, std::optional
   TORCH_CHECK(q_start.numel() >= B + 1 && tile_row.numel() >= tile_seq.numel(), "q_start / tile maps too short");
   check_same_device(out, {&q_start, &tile_seq, &tile_row});
   TORCH_CHECK(waves == 4 || (waves == 8 && tile_rows == 256), "waves must be 4, or 8 with tiles of 256 rows");
-  TORCH_CHECK(parts > 0 && tile_seq.numel() * 2 * p.Hkv * std::max<int64_t>(parts, 32) < (1LL << 31) &&
+  TORCH_CHECK(parts > 0 && parts < 65536 &&
+                  tile_seq.numel() * (tile_rows / (32 * waves)) * p.Hkv * (parts > 1 ? std::max<int64_t>(parts, 64) : 1) < (1LL << 23) &&
                   out.size(0) * G < (1LL << 31),
-              "too many rows");
+              "too many rows for a call");
   // split tiles: per (tile, part, kv head) and row 128 sums, then all rows' maxima, then all rows' sums
   p.num_parts = parts;
   if (parts > 1) {

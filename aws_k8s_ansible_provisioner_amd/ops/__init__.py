@@ -312,7 +312,7 @@ def _check_scaled(k_cache, v_cache, scales) -> None:
     """The checks of csrc/ops.cpp check_scaled for CPU tensors."""
     if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
         raise RuntimeError("scaled cache: uint8 K and V (e4m3 codes)")
-    if k_cache.dim() != 4 or not k_cache.shape[0] or k_cache.shape[2] % 32 or k_cache.shape[3] % 32:
+    if k_cache.dim() != 4 or not k_cache.numel() or k_cache.shape[2] % 32 or k_cache.shape[3] % 32:
         raise RuntimeError("scaled cache: K [NB, Hkv, BS, D], block size a multiple of 32")
     NB, H, BS, D = k_cache.shape
     if tuple(v_cache.shape) != (NB, H, BS // 8, D, 8):
@@ -386,8 +386,8 @@ def scaled_attention_decode(out, q, k_cache, v_cache, scales, block_tables, seq_
                             scale: float, workspace=None, num_parts: int = 1, part_size: int = 512,
                             q_start=None):
     """paged_attention_decode over a scaled cache: one row per sequence (row q_start[b], or b) over its
-    seq_lens[b] keys.  num_parts * part_size must hold the longest sequence's keys.  A key of a block table entry outside the cache is left out; a row that sees no
-    key is zero."""
+    seq_lens[b] keys.  num_parts * part_size must hold the longest sequence's keys.
+    A key of a block table entry outside the cache is left out; a row that sees no key is zero."""
     if _native(q):
         if workspace is None:
             workspace = _decode_workspace(seq_lens.numel(), k_cache.shape[1], gqa_group, num_parts, q.device)

@@ -197,6 +197,8 @@ def refusals(dev):
     for bad in (dict(G=1), dict(H=6), dict(nd=3), dict(qr=3), dict(qr=-2), dict(pos=pos.int()), dict(sl=sl.int()),
                 dict(sl=sl[:1]), dict(pos=pos[:1]), dict(s=s[:, :1]), dict(v=v.view(torch.int8))):
         refused(app(**bad))
+    # no kv heads
+    refused(app(k=k[:, :0], v=v[:, :0], s=s[:, :, :0], H=8, G=0))
     # no blocks of 48 tokens
     refused(app(k=torch.zeros(2, 2, 48, D, dtype=torch.uint8, device=dev),
                 v=torch.zeros(2, 2, 6, D, 8, dtype=torch.uint8, device=dev), s=torch.ones(2, 2, 2, device=dev)))

@@ -110,6 +110,18 @@ def test_refusals_gpu():
     refusals(DEV)
 
 
+def test_rows_beyond_a_launch_are_refused():
+    """As many rows as a grid cannot hold: one row, seen 2^26 times."""
+    n = 1 << 26
+    k, v = (torch.zeros(*shape, dtype=torch.uint8, device=DEV) for shape in ((1, 1, 32, D), (1, 1, 4, D, 8)))
+    s = ops.scaled_cache_scales(1, 1, 1, DEV)[0]
+    qkv = torch.zeros(1, 3 * D, dtype=torch.bfloat16, device=DEV).expand(n, -1)
+    at, cs = torch.full((n,), -1, device=DEV), torch.zeros(4, D, device=DEV)
+    q = torch.empty(0, 1, D, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        ops.scaled_cache_append(qkv, q, k, v, s, at, at, cs, None, None, 1, 1, 1e-6, decode=True, q_rows=0)
+
+
 # ------------------------------------------------------------------------------------------------ decode
 def run_decode(c, lens, H, G, parts=1, size=1024, scale=0.1, workspace=None):
     q, k, v, s, t, n, start = gpu(*c)
