@@ -643,19 +643,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
                       (kvh * G + hig) * D + 8 * h;
 #pragma unroll
     for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const bf16x8*>(src + 16 * s);
-    if (prep) {
+    if (prep) {       // (as norm_rotate does it, in the same order)
+#pragma clang fp contract(off)
       float x[8][8];
 #pragma unroll
       for (int s = 0; s < 8; ++s)
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[s][j] = bf2f(qf[s][j]);
       if (p.q_w != nullptr) {
-        float ss = 0.f;
+        float ss[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) ss += x[s][j] * x[s][j];
-        const float inv = rsqrtf(half_sum(ss) * (1.f / D) + p.eps);
+        for (int s = 0; s < 8; ++s) ss[s] = half_sum(squares(x[s]));
+        const float inv = rsqrtf((((ss[0] + ss[1]) + (ss[2] + ss[3])) + ((ss[4] + ss[5]) + (ss[6] + ss[7]))) * (1.f / D) + p.eps);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
           const bf16x8 nw = *reinterpret_cast<const bf16x8*>(p.q_w + 16 * s + 8 * h);

@@ -67,13 +67,19 @@ __device__ __forceinline__ bf16x8 codes_wide(uint32_t lo, uint32_t hi, float sca
 __device__ __forceinline__ float pair_half(float v) {    // row_ror:8: lane ^ 8, which holds the other half's dims
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, false));
 }
-// Norm (optional), then the rotation (optional) of dims d and d + 64 by c and s, in fp32 throughout.
+__device__ __forceinline__ float squares(const float (&x)[8]) {
+#pragma clang fp contract(off)
+  return (((x[0] * x[0] + x[1] * x[1]) + x[2] * x[2]) + x[3] * x[3]) +
+         (((x[4] * x[4] + x[5] * x[5]) + x[6] * x[6]) + x[7] * x[7]);
+}
+// Norm (optional), then the rotation (optional) of dims d and d + 64 by c and s, in fp32 throughout.  Every product and
+// sum is rounded by itself, squares are added by fours and those in pairs, as whole tensors' arithmetic does it: an
+// entry that lies between two codes would fall to the other side of that form's once in a million, half a code away.
 __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const bf16x8& w, bool rotate, const f32x4 (&c)[2],
                                             const f32x4 (&s)[2], int li, float eps) {
+#pragma clang fp contract(off)
   if (norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    float ss = squares(x);
     ss += dpp_mov<0xB1>(ss);
     ss += dpp_mov<0x4E>(ss);
     ss += dpp_mov<0x141>(ss);
