@@ -654,7 +654,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
         float ss[8];
 #pragma unroll
         for (int s = 0; s < 8; ++s) ss[s] = half_sum(squares(x[s]));
-        const float inv = rsqrtf((((ss[0] + ss[1]) + (ss[2] + ss[3])) + ((ss[4] + ss[5]) + (ss[6] + ss[7]))) * (1.f / D) + p.eps);
+        const float inv = inv_sqrt((((ss[0] + ss[1]) + (ss[2] + ss[3])) + ((ss[4] + ss[5]) + (ss[6] + ss[7]))) * (1.f / D) + p.eps);
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
           const bf16x8 nw = *reinterpret_cast<const bf16x8*>(p.q_w + 16 * s + 8 * h);

@@ -72,6 +72,12 @@ __device__ __forceinline__ float squares(const float (&x)[8]) {
   return (((x[0] * x[0] + x[1] * x[1]) + x[2] * x[2]) + x[3] * x[3]) +
          (((x[4] * x[4] + x[5] * x[5]) + x[6] * x[6]) + x[7] * x[7]);
 }
+// 1 / sqrt(m) to the nearest: a Newton step from the instruction's, whose error is up to one unit in the last place
+__device__ __forceinline__ float inv_sqrt(float m) {
+  const float y = rsqrtf(m), r = m * y;
+  const float e = fmaf(-fmaf(m, y, -r), y, fmaf(-r, y, 1.f));
+  return m > 0.f && m < INFINITY ? fmaf(0.5f * e, y, y) : y;
+}
 // Norm (optional), then the rotation (optional) of dims d and d + 64 by c and s, in fp32 throughout.  Every product and
 // sum is rounded by itself, squares are added by fours and those in pairs, as whole tensors' arithmetic does it: an
 // entry that lies between two codes would fall to the other side of that form's once in a million, half a code away.
@@ -84,7 +90,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[8], bool norm, const bf16
     ss += dpp_mov<0x4E>(ss);
     ss += dpp_mov<0x141>(ss);
     ss += dpp_mov<0x140>(ss);
-    const float inv = rsqrtf(ss * (1.f / 128) + eps);
+    const float inv = inv_sqrt(ss * (1.f / 128) + eps);
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * bf2f(w[e]);
   }

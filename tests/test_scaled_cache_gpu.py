@@ -74,6 +74,41 @@ def test_append_some_query_rows_and_no_rotation():
     assert bool((q[3:] == 7).all())
 
 
+def test_append_rows_whose_squares_overflow():
+    """The norm of such a row is infinite, its entries zeros; rows of zeros stay zeros."""
+    qkv, k, v, s, pos, sl, cs, w = make(24, 2, 1, 3, [8, 9, 10], 32, 2, True)
+    qkv[0, :3 * D] = 2.0 ** 100
+    qkv[1, :3 * D] = 0
+    k1, v1, s1, q = run_append((qkv, k, v, s, pos, sl, cs, w), 2, 1, range(3))
+    assert not q[:2].any() and torch.isfinite(q[2].float()).all()
+    assert not orc.codes(k1, v1)[0, 0, 0, 8:10].any()
+
+
+def test_append_rounds_as_whole_tensors_do():
+    """Norm and rotation by torch's operations in fp32 on the GPU, each rounded by itself: the same query rows and the
+    same codes, but for what another order of the sum of squares could move: a few units of 2^-24 against a bf16 step of 2^-8
+    or more, less than one entry in 10000."""
+    T, H, G = 640, 8, 2
+    qkv, k, v, s, pos, sl, cs, w = gpu(*make(25, H, G, T, list(range(T)), 32, T // 32, True)[:7], None)
+    w = [torch.randn(D, device=DEV).bfloat16() for _ in range(2)]
+    q = torch.empty(T, H, D, dtype=torch.bfloat16, device=DEV)
+    ops.scaled_cache_append(qkv, q, k, v, s, pos, sl, cs, *w, H, G, 1e-6)
+    x = qkv.float()[:, :(H + 2 * G) * D].view(T, -1, D)
+    a = cs[pos][:, None]
+
+    def turned(y, u):
+        y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-6) * u.float()
+        lo, hi = y[..., :64], y[..., 64:]
+        return torch.cat([lo * a[..., :64] - hi * a[..., 64:], hi * a[..., :64] + lo * a[..., 64:]], -1)
+
+    assert int((turned(x[:, :H], w[0]).bfloat16() != q).sum()) <= q.numel() // 10000
+    want = turned(x[:, H:H + G], w[1])
+    got = orc.codes(k.cpu(), v.cpu())[0].transpose(1, 2).reshape(T, G, D)
+    scale = s[0].repeat_interleave(32, 0)[:, :, None]
+    codes = (want / scale).clamp(-448, 448).to(torch.float8_e4m3fn).double().cpu()
+    assert int((codes != got).sum()) <= got.numel() // 10000
+
+
 def test_append_rows_that_are_not_finite():
     case = make(23, 2, 1, 5, [60, 61, 62, 63, 64], 32, 4, False)
     qkv = case[0]
