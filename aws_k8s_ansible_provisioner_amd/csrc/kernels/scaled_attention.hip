@@ -515,8 +515,13 @@ __device__ __forceinline__ float half_sum(float x) {
 __device__ __forceinline__ int row_key(int r) { return 16 * (r >> 4) + 8 * ((r >> 2) & 1) + 4 * ((r >> 3) & 1) + (r & 3); }
 
 constexpr int kKeys = 64;
-// Key tiles that a part of a split tile takes at least: 700 tokens behind 300 (16 / 8 heads) 28 us, with 8 36.5; 1500 of
-// one kv head of 8 29 and 37.
+// Fragments asked for ahead of the product that takes them.  (Left to the compiler each was read right before its
+// product and waited for: 1000 tokens behind 9000 in one part, a wave to a SIMD, 292 us; 3 ahead 235, 4 and 6 too.)
+constexpr int kAhead = 3;
+// Vector and matrix instructions and LDS stay on their side; scalar ones and loads may cross.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0x14); }
+// Key tiles that a part of a split tile takes at least (with 8, and all at once before the products: 700 tokens behind
+// 300, 16 / 8 heads, 36.5 us for 28).
 constexpr int kSplitTiles = 4;
 
 // key tiles of a tile's rows, and the parts that they are cut into
@@ -538,13 +543,15 @@ __device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int seq, int row0) 
   return t;
 }
 
-// A wave's step has two halves, with a barrier behind each: products (outputs of tile u by its weights, scores of tile
-// u + 1; beside them K of tile u + 2 and V of tile u + 1 are widened into LDS, where their buffers are free, and the
-// next ones asked for) and the weights of the next tile.  Of eight waves the later four go half a step behind: the two
-// waves of a SIMD are in different halves, one's products beside the other's exponentials.
+// A wave's step, a barrier behind it: 16 products for the outputs by tile u - 1's weights, between them the maximum of
+// tile u's scores, and K of tile u + 2 and V of tile u widened into LDS, where their buffers are free; then 16
+// products for the scores of tile u + 1, between them the weights of tile u.  Products and what stands between them are
+// laid down one by one (fence): a SIMD issues in order, and a product runs 32 cycles beside the next vector work.
+// Before, with all products of a step and then all weights, and eight waves' later four half a step behind: 1000 behind
+// 9000 in one part, four waves 292 us (now 198), eight 264 (241); 2 of ~759 (20 / 4 heads) 30.5 (23.3); 4 of 4096 (32 /
+// 8) 569 (528).  One wave of 64 rows, whose fragments serve two products: 448 for the 264.
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p, int subs) {
-  constexpr bool LATE = NW == 8;
   constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
   __shared__ __attribute__((aligned(16))) bf16 lds[2][2][kKeys * D];    // [K | V][buffer]
   const int flat = gridDim.x - 1 - blockIdx.x;     // the map rises by work: longest tiles first
@@ -598,16 +605,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
       to[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, ((tid * PW + i) & 255) * 16, 0, 0));
   };
   // K image: token rows of 256 bytes, 16-byte column c of row k at c ^ (k & 15); V image: the groups as they are
-  auto store_k = [&](int buf, float scale) {
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      const int pc = (tid * PW + i) & 255;       // K: [half 2][dims / 32 4][row 16][2]
-      const int col = 4 * ((pc >> 5) & 3) + 2 * (pc & 1), r16 = (pc >> 1) & 15;
-      const int key = 32 * chunk + 8 * (r16 >> 2) + 4 * (pc >> 7) + (r16 & 3);
-      bf16* kl = lds[0][buf] + key * D;
-      *reinterpret_cast<bf16x8*>(kl + (col ^ (key & 15)) * 8) = codes_wide(kc[i][0], kc[i][1], scale);
-      *reinterpret_cast<bf16x8*>(kl + ((col + 1) ^ (key & 15)) * 8) = codes_wide(kc[i][2], kc[i][3], scale);
-    }
+  auto put_k = [&](int buf, float scale, int n) {      // n: half a piece
+    const int i = n >> 1, pc = (tid * PW + i) & 255;       // K: [half 2][dims / 32 4][row 16][2]
+    const int col = 4 * ((pc >> 5) & 3) + 2 * (pc & 1) + (n & 1), r16 = (pc >> 1) & 15;
+    const int key = 32 * chunk + 8 * (r16 >> 2) + 4 * (pc >> 7) + (r16 & 3);
+    *reinterpret_cast<bf16x8*>(lds[0][buf] + key * D + (col ^ (key & 15)) * 8) =
+        codes_wide(kc[i][2 * (n & 1)], kc[i][2 * (n & 1) + 1], scale);
   };
   // values behind the last key may be no numbers: zeros
   auto clear_v = [&](int t) {
@@ -621,13 +624,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
       vc[i] = u32x4{vc[i][0] & lo, vc[i][1] & hi, vc[i][2] & lo, vc[i][3] & hi};
     }
   };
-  auto store_v = [&](int buf, float scale) {
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-      bf16* vl = lds[1][buf] + (chunk * 256 + ((tid * PW + i) & 255)) * 16;
-      *reinterpret_cast<bf16x8*>(vl) = codes_wide(vc[i][0], vc[i][1], scale);
-      *reinterpret_cast<bf16x8*>(vl + 8) = codes_wide(vc[i][2], vc[i][3], scale);
-    }
+  auto put_v = [&](int buf, float scale, int n) {
+    const int i = n >> 1;
+    *reinterpret_cast<bf16x8*>(lds[1][buf] + (chunk * 256 + ((tid * PW + i) & 255)) * 16 + 8 * (n & 1)) =
+        codes_wide(vc[i][2 * (n & 1)], vc[i][2 * (n & 1) + 1], scale);
   };
 
   fetch(kc, p.k_cache, ta);
@@ -674,22 +674,22 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
         }
     }
   }
-  store_k(ta & 1, kscale_of(ta));
-  clear_v(ta);
-  store_v(ta & 1, vscale_of(ta));
+#pragma unroll
+  for (int n = 0; n < 2 * PW; ++n) put_k(ta & 1, kscale_of(ta), n);
 #pragma unroll
   for (int i = 0; i < PW; ++i) kc[i] = kc2[i];
-  store_k((ta + 1) & 1, kscale_of(ta + 1));
+#pragma unroll
+  for (int n = 0; n < 2 * PW; ++n) put_k((ta + 1) & 1, kscale_of(ta + 1), n);
   fetch(kc, p.k_cache, ta + 2);
-  fetch(vc, p.v_cache, ta + 1);
+  // (no tile before the first: weights and values of zero)
+#pragma unroll
+  for (int i = 0; i < 2 * PW; ++i) *reinterpret_cast<u32x4*>(lds[1][(ta + 1) & 1] + (tid * 2 * PW + i) * 8) = u32x4{};
 
-  f32x16 o[4], s[2];
+  f32x16 o[4], sa[2], sb[2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  for (int i = 0; i < 4; ++i) o[i] = f32x16{};
   float m = -1e30f, l = 0.f;
-  bf16x8 pb[4];                    // weights: keys 16 g + 8 h .. + 7
+  bf16x8 pb[4] = {};                    // weights: keys 16 g + 8 h .. + 7
   auto k_frag = [&](int buf, int i, int k) {
     const int key = 32 * k + row_key(r);
     return *reinterpret_cast<const bf16x8*>(lds[0][buf] + key * D + ((2 * i + h) ^ (key & 15)) * 8);
@@ -703,99 +703,143 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  auto scores = [&](int i, int buf) {
-    s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(buf, i >> 1, i & 1), qf[i >> 1], s[i & 1], 0, 0, 0);
-  };
-  auto rows = [&](int i, int buf) {
-    o[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v_frag(buf, i >> 2, i & 3), pb[i >> 2], o[i & 3], 0, 0, 0);
-  };
-  auto zero = [&]() {
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[k][j] = 0.f;
-  };
-  const bool late = LATE && w >= 4;
-  half();
-  if (late) half();
-  zero();
-#pragma unroll
-  for (int i = 0; i < 16; ++i) scores(i, ta & 1);
-  half();
-  // weights of tile u from its scores
-  auto weigh = [&](int u) {
-    {
-      const int t = u, key0 = t * kKeys;
-      const bool lost0 = page_of(t, 0) < 0, lost1 = page_of(t, 1) < 0;
-      if (key0 + kKeys - 1 > w_min || lost0 || lost1) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || (k ? lost1 : lost0)) s[k][j] = -INFINITY;
-      }
-      float tp[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  auto mask = [&](f32x16 (&s)[2], int t) {
+    const int key0 = t * kKeys;
+    const bool lost0 = page_of(t, 0) < 0, lost1 = page_of(t, 1) < 0;
+    if (key0 + kKeys - 1 > w_min || lost0 || lost1) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) tp[j & 3] = fmaxf(tp[j & 3], s[k][j]);
+        for (int j = 0; j < 16; ++j)
+          if (key0 + 32 * k + 16 * (j >> 3) + 8 * h + (j & 7) > limit || (k ? lost1 : lost0)) s[k][j] = -INFINITY;
+    }
+  };
+  float a = 1.f;
+  // 16 products each, behind the n-th beside(n)
+  auto rows = [&](int buf, const auto& beside) {
+    bf16x8 f[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) f[n] = v_frag(buf, n >> 2, n & 3);
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      fence();
+      o[n & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[n % kAhead], pb[n >> 2], o[n & 3], 0, 0, 0);
+      if (n + kAhead < 16) f[n % kAhead] = v_frag(buf, (n + kAhead) >> 2, (n + kAhead) & 3);
+      beside(n);
+    }
+    fence();
+  };
+  auto scores = [&](f32x16 (&s)[2], int buf, const auto& beside) {
+    bf16x8 f[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) f[n] = k_frag(buf, n >> 1, n & 1);
+    s[0] = f32x16{};
+    s[1] = f32x16{};
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+      fence();
+      s[n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[n % kAhead], qf[n >> 1], s[n & 1], 0, 0, 0);
+      if (n + kAhead < 16) f[n % kAhead] = k_frag(buf, (n + kAhead) >> 1, (n + kAhead) & 1);
+      beside(n);
+    }
+    fence();
+  };
+  // a tile's maximum, four scores at a time, then what its weights are relative to
+  float tp[4];
+  bool moved = false;
+  auto tops = [&](const f32x16 (&s)[2], int n) {
+    if (n < 8) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = s[n >> 2][4 * (n & 3) + j];
+        tp[j] = n == 0 ? x : fmaxf(tp[j], x);
+      }
+    } else if (n == 8) {
       const float top = fmaxf(fmaxf(tp[0], tp[1]), fmaxf(tp[2], tp[3]));
       // the maximum moves, and sums are scaled, only where it is exceeded by 2^8: weights up to that are as good
       const float cand = fmaxf(m, half_max(top) * p.scale_log2), mn = cand > m + 8.f ? cand : m;
-      const float a = __builtin_amdgcn_exp2f(m - mn);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[k][j], p.scale_log2, -mn));
-          sum[j & 3] += e;
-          pb[2 * k + (j >> 3)][j & 7] = f2bf(e);
-        }
-      l = l * a + half_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
-      if (__any(mn != m)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[i][j] *= a;
-      }
+      a = __builtin_amdgcn_exp2f(m - mn);
+      moved = mn != m;
       m = mn;
     }
   };
-  for (int u = ta; u + 1 < tb; ++u) {
-    weigh(u);
-    clear_v(u + 1);
-    if (u + 3 - held > 31) hold(u);
-    half();
-    if constexpr (LATE) __builtin_amdgcn_s_setprio(1);
-    zero();
+  float sum[4], x0[2], e0[2];
+  // two weights of 32: arguments one call ahead of the exponentials, sums one behind
+  auto weigh = [&](const f32x16 (&s)[2], int n) {
+    if (n == 0) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      scores(i, (u + 1) & 1);
-      rows(i, u & 1);
+      for (int j = 0; j < 4; ++j) sum[j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) x0[j] = fmaf(s[0][j], p.scale_log2, -m);
     }
-    // (behind the last tile: zeros, of which nothing is made)
-    store_k(u & 1, kscale_of(u + 2));
-    store_v((u + 1) & 1, vscale_of(u + 1));
-    fetch(kc, p.k_cache, u + 3);
-    fetch(vc, p.v_cache, u + 2);
-    if constexpr (!LATE) {      // (keeps the four-wave form's registers: left to itself it spills 44 bytes)
-      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+    if (n > 0) {
+      const int e = 2 * (n - 1);
 #pragma unroll
-      for (int i = 0; i < 12; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+      for (int j = 0; j < 2; ++j) {
+        sum[(e + j) & 3] += e0[j];
+        pb[e >> 3][(e & 7) + j] = f2bf(e0[j]);
       }
     }
-    if constexpr (LATE) __builtin_amdgcn_s_setprio(0);
-    half();
-  }
-  weigh(tb - 1);
-  half();
+    if (n < 16) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) rows(i, (tb - 1) & 1);
-  if (LATE && !late) half();
+      for (int j = 0; j < 2; ++j) e0[j] = __builtin_amdgcn_exp2f(x0[j]);
+      if (n < 15) {
+        const int e = 2 * (n + 1);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x0[j] = fmaf(s[e >> 4][(e & 15) + j], p.scale_log2, -m);
+      }
+    } else {
+      l = l * a + half_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    }
+  };
+  auto settle = [&]() {
+    if (__any(moved)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] *= a;
+    }
+  };
+  auto none = [](int) {};
+  half();
+  scores(sa, ta & 1, none);
+  half();
+  auto step = [&](int u, f32x16 (&s)[2], f32x16 (&sn)[2]) {
+    mask(s, u);
+    clear_v(u);
+    if (u + 3 - held > 31) hold(u);
+    const float ksc = kscale_of(u + 2), vsc = vscale_of(u);
+    rows((u + 1) & 1, [&](int n) {
+      tops(s, n);
+      if (n >= 16 - 4 * PW && n < 16 - 2 * PW) put_k(u & 1, ksc, n - 16 + 4 * PW);
+      if (n >= 16 - 2 * PW) put_v(u & 1, vsc, n - 16 + 2 * PW);
+    });
+    fetch(kc, p.k_cache, u + 3);
+    fetch(vc, p.v_cache, u + 1);
+    settle();
+    scores(sn, (u + 1) & 1, [&](int n) { weigh(s, n); });
+    weigh(s, 16);
+    half();
+  };
+  int u = ta;
+  for (; u + 2 < tb; u += 2) {
+    step(u, sa, sb);
+    step(u + 1, sb, sa);
+  }
+  if (u + 1 < tb) {
+    step(u, sa, sb);
+    sa[0] = sb[0];
+    sa[1] = sb[1];
+  }
+  mask(sa, tb - 1);
+  clear_v(tb - 1);
+  rows(tb & 1, [&](int n) {
+    tops(sa, n);
+    if (n >= 8 && n < 8 + 2 * PW) put_v((tb - 1) & 1, vscale_of(tb - 1), n - 8);
+  });
+  settle();
+#pragma unroll
+  for (int n = 0; n <= 16; ++n) weigh(sa, n);
+  half();
+  rows((tb - 1) & 1, none);
   // dims 32 dt + 8 i + 4 h .. + 3 of a row to a lane
   if (T.parts > 1) {
     const int64_t at = ((int64_t)(tile * p.num_parts + part) * p.Hkv + kvh) * ROWS + 32 * w + r;

@@ -444,13 +444,14 @@ def scaled_attention_decode_fused(out, qkv, k_cache, v_cache, scales, block_tabl
 def scaled_prefill_plan(tiles: int, tile_rows: int, max_len: int) -> tuple[int, int]:
     """(waves of a workgroup, parts along the keys) for prompt tiles, times kv heads, of sequences of at most
     max_len keys.  Eight waves take a tile of 256 rows whole; where sequences are short, or the tiles few and the
-    keys not many, two workgroups of four do better: 24 prompts of ~250 (32 / 4 heads) 68 us, with eight waves 72,
-    4 of ~400 (16 / 8) 20.8 and 23.3, 700 tokens behind 300 27.8 and 30.7; but 2 of 1500 (32 / 8) 60 and 54, 8 of
-    2048 356 and 327, 1000 behind 9000 (16 / 8) 111 and 98.  Parts: as many as fill the card, one workgroup of eight
-    waves or two of four to a CU, of 512 keys or more as far as the host knows."""
-    waves = 8 if tile_rows == 256 and max_len > 512 and not (tiles < 128 and max_len <= 4096) else 4
+    keys not many, two workgroups of four do better: 24 prompts of ~250 (32 / 4 heads) 41 us, with eight waves 46,
+    2 of 1000 (32 / 8) 31.9 and 36.3, one of 2000 (16 / 8) 42.7 and 47.9; but 2 of 1500 (32 / 8) 59 and 51, 8 of
+    2048 337 and 312, 1000 behind 9000 (16 / 8) 98 and 91.  Parts: as many as fill the card, one workgroup of eight
+    waves or two of four to a CU, of 448 keys or more as far as the host knows (one of 1000, 16 / 8 heads, in two
+    24.7 us, whole 25.9; of 700 20.3 and 20.1)."""
+    waves = 8 if tile_rows == 256 and max_len > 512 and not (tiles <= 256 and max_len <= 4096) else 4
     grid = tiles * tile_rows // (32 * waves)
-    return waves, max(1, min((256 if waves == 8 else 512) // max(grid, 1), max_len // 512, 16))
+    return waves, max(1, min((256 if waves == 8 else 512) // max(grid, 1), max_len // 448, 16))
 
 
 def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq_lens, q_start, tile_seq,

@@ -260,7 +260,7 @@ def test_prompt_plans():
             for n in (1, 500, 1000, 5000, 100000):
                 waves, parts = ops.scaled_prefill_plan(tiles, rows, n)
                 assert waves in (4, 8) and 32 * waves <= rows and 1 <= parts <= 16
-                assert parts == 1 or n >= 1024
+                assert parts == 1 or n >= 896
 
 
 def test_engine_refuses_roles_and_blocks():

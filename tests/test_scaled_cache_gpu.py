@@ -255,7 +255,7 @@ def test_prompt_forms():
     """What FORMS stand for, for few tiles."""
     assert [ops.scaled_prefill_plan(4, r, n) for r, n in ((128, 500), (128, 100000), (256, 500), (256, 2000),
                                                           (256, 100000))] == \
-        [(4, 1), (4, 16), (4, 1), (4, 3), (8, 16)]
+        [(4, 1), (4, 16), (4, 1), (4, 4), (8, 16)]
     assert ops.scaled_prefill_plan(4096, 256, 2048) == (8, 1) and ops.scaled_prefill_plan(64, 256, 10016) == (8, 4)
 
 
