@@ -29,6 +29,9 @@ __device__ __forceinline__ int keys_of(const ScaledAttn& p, int seq) {
 // 64 p + 16 g .. + 15 of a token (its k-steps 2 p and 2 p + 1 contract over the first and second 8, q in the same
 // order), of V two dims of an 8-token group.  The next chunk's K is asked for when this one's scores are formed, its
 // V when this one's is used up: a whole chunk on the way in the registers of one.
+// Rows that fill the card are bound by their codes' bytes: 200 rows of up to 4000 keys (16 / 8 heads) 221 us, 6.1 TB/s,
+// 64 of up to 2048 (32 / 8) 35.3, 5.6; few by a chain of loads: one at 333 5.5 us in a graph, 3 of up to 30000 of one kv
+// head 15.8, of which the merge within the launch 3.
 struct Chunk {
   u32x4 k[2][2];   // [16-token tile][p]
   u32x4 v[4];      // dims 32 n + 2 r and + 1 of group g
@@ -550,6 +553,8 @@ __device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int seq, int row0) 
 // Before, with all products of a step and then all weights, and eight waves' later four half a step behind: 1000 behind
 // 9000 in one part, four waves 292 us (now 198), eight 264 (241); 2 of ~759 (20 / 4 heads) 30.5 (23.3); 4 of 4096 (32 /
 // 8) 569 (528).  One wave of 64 rows, whose fragments serve two products: 448 for the 264.
+// Bound by vector work and power: 8 prompts of 2048 (32 / 8 heads) 311 us, 0.88 PFLOP/s, a CU's tile of 256 rows by 64
+// keys in 2.0 us, where the products of a SIMD are 2048 cycles and the vector work of its two waves 2500.
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p, int subs) {
   constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
@@ -870,7 +875,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
     }
 }
 
-// The parts of split tiles: 32 threads to a row, 8 rows to a workgroup.
+// The parts of split tiles: 32 threads to a row, 8 rows to a workgroup.  Bound by the parts' bytes: 16000 rows in four
+// parts 8.2 us, 4.1 TB/s.
 template <int ROWS>
 __global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p, int subs) {
   const int item = blockIdx.x / (ROWS / 8), sub = blockIdx.x - item * (ROWS / 8);

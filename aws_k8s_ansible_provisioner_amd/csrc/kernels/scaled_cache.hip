@@ -6,6 +6,8 @@
 // Rows whose slots follow each other inside a page are a run, its first row the leader; a workgroup looks over a span
 // of 8 to 32 rows of the batch for leaders (a wave over one, where rows are single tokens of their sequences) and
 // takes each run: magnitudes first, then the codes.  The caller keeps the rows of a page together, in rising slots.
+// Many rows are bound by their bytes (11881 of 32 / 8 heads 58 us, 4.7 TB/s), few by a chain of loads: slots, positions,
+// angles (one row 4.4 us in a graph).
 #include "scaled_cache.h"
 #include "kernels.h"
 
