@@ -317,6 +317,16 @@ def test_prompts_of_no_visible_keys(rows, max_len):
     assert not out.any()
 
 
+@pytest.mark.parametrize("waves,parts", [(4, 1), (8, 1), (4, 2), (8, 3)])
+@pytest.mark.parametrize("page", [32, 96])
+def test_prompts_of_many_key_tiles(waves, parts, page, monkeypatch):
+    """More tiles of 64 keys in a part than the pages a wave looks up at once, even and odd ones."""
+    lens, new = [4500, 2113, 33, 1985], [3, 70, 33, 1]
+    c = attention_case(46, 2, 1, page, lens, new)
+    monkeypatch.setattr(ops, "scaled_prefill_plan", lambda *a: (waves, parts))
+    close(run_prompt(c, lens, new, 2, 1, 32 * waves), *want_rows(c, lens))
+
+
 def test_prompts_leave_other_rows():
     """Sequences that no tile names (a mixed step's single tokens) keep their rows."""
     lens, new = [40, 100, 64], [1, 60, 64]
