@@ -876,7 +876,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kerne
 }
 
 // The parts of split tiles: 32 threads to a row, 8 rows to a workgroup.  Bound by the parts' bytes: 16000 rows in four
-// parts 8.2 us, 4.1 TB/s.
+// parts 8.0 us, 4.2 TB/s (one part after the other 8.3).
 template <int ROWS>
 __global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p, int subs) {
   const int item = blockIdx.x / (ROWS / 8), sub = blockIdx.x - item * (ROWS / 8);
@@ -888,13 +888,29 @@ __global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p,
   if (pos >= T.q_len) return;
   float M = -1e30f, L = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < T.parts; ++i) {
-    const int64_t at = ((int64_t)(tile * p.num_parts + i) * p.Hkv + kvh) * ROWS + row;
-    const float m = p.part_m[at], mn = fmaxf(M, m);
-    const float a = __builtin_amdgcn_exp2f(M - mn), b = __builtin_amdgcn_exp2f(m - mn);
-    acc = acc * a + *reinterpret_cast<const f32x4*>(p.part_o + at * D + d0) * b;
-    L = L * a + p.part_l[at] * b;
-    M = mn;
+  constexpr int U = 4;             // parts asked for together
+  for (int i0 = 0; i0 < T.parts; i0 += U) {
+    float m[U], l[U], top = M;
+    f32x4 o[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = ((int64_t)(tile * p.num_parts + min(i0 + u, T.parts - 1)) * p.Hkv + kvh) * ROWS + row;
+      m[u] = p.part_m[at];
+      l[u] = p.part_l[at];
+      o[u] = *reinterpret_cast<const f32x4*>(p.part_o + at * D + d0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) top = fmaxf(top, m[u]);     // (the last part again changes nothing)
+    const float a = __builtin_amdgcn_exp2f(M - top);
+    M = top;
+    L *= a;
+    acc *= a;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float b = i0 + u < T.parts ? __builtin_amdgcn_exp2f(m[u] - M) : 0.f;
+      L += b * l[u];
+      acc += b * o[u];
+    }
   }
   const float inv = L > 0.f ? 1.f / L : 0.f;
   bf16x4 x;
