@@ -314,12 +314,14 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
 void launch_scaled_append(const ScaledAppend& p, hipStream_t s) {
   const long per = 2 * p.Hkv;
   const long single = (p.singles * per + 3) / 4;
-  // Runs begin anywhere, and a span's are taken in turn: the smallest span of 8, 16 or 32 rows whose workgroups are
-  // at most 512, two to a unit.  8 kv heads, spans of 8, 16 and 32: 49 sequences of 3 tokens 8.2, 12.8 and 20.7 us; 8
-  // of ~130 10.0, 9.0 and 11.8; one of 1000 9.4, 7.7 and 6.9; 60 of ~200 46.4, 38.5 and 36.9.
-  int rows = 8;
-  while (rows < 32 && (long)(p.T - p.singles + rows - 1) / rows * p.Hkv > 512) rows *= 2;
-  const long runs = (long)(p.T - p.singles + rows - 1) / rows * p.Hkv;
+  // Runs begin anywhere, and a span's are taken in turn: spans of 8 rows where their workgroups are at most 512, two to a
+  // unit, of 16 up to 1300, else of 32.  8 kv heads, spans of 8, 16 and 32: 49 sequences of 3 tokens 8.2, 12.8 and 20.7
+  // us; 8 of ~130 10.0, 9.0 and 11.8; one of 1000 9.4, 7.7 and 6.9; 40 of ~40 11.5, 11.0 and 12.4; 60 of ~200 46.4, 38.5
+  // and 36.9; 4 kv heads, 24 of ~210 in blocks of 64 14.5, 12.1 and 14.6.
+  const long rest = p.T - p.singles;
+  auto spans = [&](int rows) { return (rest + rows - 1) / rows * p.Hkv; };
+  const int rows = spans(8) <= 512 ? 8 : spans(16) <= 1300 ? 16 : 32;
+  const long runs = spans(rows);
   const long q = ((long)p.q_rows * ((p.Hq + kQHeads - 1) / kQHeads) + 15) / 16;
   if (single + runs + q == 0) return;
   const dim3 grid((unsigned)(single + runs + q));

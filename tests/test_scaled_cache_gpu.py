@@ -48,7 +48,7 @@ def run_append(case, H, G, slots, decode=False, num_decode=0, q_rows=-1, rope=Tr
     (2, 2, 64, 9, list(range(7, 64)) + list(range(130, 192)) + list(range(320, 384)), False),
     (1, 1, 256, 4, list(range(300, 700)), True),
     (8, 8, 32, 60, [i for b in range(7) for i in range(200 * b + 5, 200 * b + 5 + 85)], True),   # spans of 16 rows
-    (8, 8, 32, 110, list(range(40, 2200)), False),                                               # of 32
+    (8, 8, 32, 110, list(range(40, 2700)), False),                                               # of 32
     (2, 1, 64, 40, [64 * i + 60 - i % 3 + j for i in range(30) for j in range(1 + i % 4)], True),  # short runs, late
 ])
 def test_append(H, G, page, pages, slots, norm):
