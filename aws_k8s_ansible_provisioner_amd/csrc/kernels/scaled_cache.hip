@@ -6,7 +6,7 @@
 // Rows whose slots follow each other inside a page are a run, its first row the leader; a workgroup looks over a span
 // of 8 to 32 rows of the batch for leaders (a wave over one, where rows are single tokens of their sequences) and
 // takes each run: magnitudes first, then the codes.  The caller keeps the rows of a page together, in rising slots.
-// Many rows are bound by their bytes (11881 of 32 / 8 heads 58 us, 4.7 TB/s), few by a chain of loads: slots, positions,
+// Many rows are bound by their bytes (11881 of 32 / 8 heads 55.6 us, 4.9 TB/s), few by a chain of loads: slots, positions,
 // angles (one row 4.4 us in a graph).
 #include "scaled_cache.h"
 #include "kernels.h"
@@ -21,12 +21,24 @@ constexpr int D = 128;
 struct Angles {
   f32x4 c[2], s[2];
 };
-__device__ __forceinline__ Angles angles(const ScaledAppend& p, int t, int li) {
+__device__ __forceinline__ int place_of(const ScaledAppend& p, int t) {      // a row's position, inside the table
   const int64_t pos = p.rope ? p.positions[t] : 0;
-  const f32x4* at = reinterpret_cast<const f32x4*>(
-      p.cos_sin + (size_t)(pos < 0 ? 0 : pos < p.max_pos ? pos : p.max_pos - 1) * D + 8 * (li & 7));
+  return (int)(pos < 0 ? 0 : pos < p.max_pos ? pos : p.max_pos - 1);
+}
+__device__ __forceinline__ Angles angles(const ScaledAppend& p, int place, int li) {
+  const f32x4* at = reinterpret_cast<const f32x4*>(p.cos_sin + (size_t)place * D + 8 * (li & 7));
   return Angles{{at[0], at[1]}, {at[16], at[17]}};
 }
+// Places of the 64 rows from `from` on, one to a lane: asked for beside their slots.  (Each row for itself, behind them:
+// 11881 rows 58.2 us for 55.6, 24 sequences of ~210 12.0 for 11.6.)
+struct Places {
+  int from, mine;
+  __device__ __forceinline__ int of(const ScaledAppend& p, int t) const {
+    int v = __shfl(mine, (t - from) & 63, 64);
+    if (t - from >= 64) v = place_of(p, t);
+    return v;
+  }
+};
 
 // q: 16 lanes per row and four of its heads
 constexpr int kQHeads = 4;
@@ -41,7 +53,7 @@ __device__ __forceinline__ void append_q(const ScaledAppend& p, int block) {
 #pragma unroll
   for (int j = 0; j < kQHeads; ++j)
     raw[j] = *reinterpret_cast<const bf16x8*>(row + min(h0 + j, p.Hq - 1) * D);
-  const Angles a = angles(p, t, li);
+  const Angles a = angles(p, place_of(p, t), li);
   const bf16x8 w = p.q_w != nullptr ? *reinterpret_cast<const bf16x8*>(p.q_w + 8 * li) : bf16x8{};
 #pragma unroll
   for (int j = 0; j < kQHeads; ++j) {
@@ -57,9 +69,10 @@ __device__ __forceinline__ void append_q(const ScaledAppend& p, int block) {
 }
 
 // dims 8 li .. + 7 of a row's key, normed and rotated
-__device__ __forceinline__ void key_row(float (&x)[8], const ScaledAppend& p, int h, int row, int li, const bf16x8& w) {
+__device__ __forceinline__ void key_row(float (&x)[8], const ScaledAppend& p, const Places& places, int h, int row, int li,
+                                        const bf16x8& w) {
   const bf16x8 raw = *reinterpret_cast<const bf16x8*>(p.qkv + (size_t)row * p.qkv_stride + (p.Hq + h) * D + 8 * li);
-  const Angles a = angles(p, row, li);
+  const Angles a = angles(p, places.of(p, row), li);
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] = bf2f(raw[e]);
   norm_rotate(x, p.k_w != nullptr, w, p.rope, a.c, a.s, li, p.eps);
@@ -105,7 +118,7 @@ __device__ __forceinline__ void put_values(uint8_t* codes, int o, int off, int n
 
 // A run of a wave of its own, keys or values: rows t .. t + n - 1 (single tokens: one, as a rule) into the page from
 // token `off` on, 4 tokens of keys or 8 of values at a time.
-__device__ __forceinline__ void append_keys(const ScaledAppend& p, int h, int t, int n, int64_t blk, int off) {
+__device__ __forceinline__ void append_keys(const ScaledAppend& p, const Places& places, int h, int t, int n, int64_t blk, int off) {
   const int lane = threadIdx.x & 63, li = lane & 15, sub = lane >> 4;
   uint8_t* codes = p.k_cache + ((size_t)blk * p.Hkv + h) * p.BS * D;
   const bf16x8 w = p.k_w != nullptr ? *reinterpret_cast<const bf16x8*>(p.k_w + 8 * li) : bf16x8{};
@@ -113,7 +126,7 @@ __device__ __forceinline__ void append_keys(const ScaledAppend& p, int h, int t,
   float x[8];
   auto load = [&](int piece) {
     const int row = t + min(max(o0 + piece * 4 + sub - off, 0), n - 1);   // (beyond the run: its first or last again)
-    key_row(x, p, h, row, li, w);
+    key_row(x, p, places, h, row, li, w);
   };
   float most = 0.f;
   for (int piece = 0; piece < pieces; ++piece) {
@@ -150,7 +163,7 @@ __device__ __forceinline__ void append_values(const ScaledAppend& p, int h, int 
 // a run's keys or values, all of its tokens one after the other, a step of 1000 rows (8 kv heads) took 15 us, of 5000
 // rows in blocks of 64 (4 kv heads) 30.
 template <int kHeld>
-__device__ __forceinline__ void append_run(const ScaledAppend& p, int h, int t, int n, int64_t blk, int off,
+__device__ __forceinline__ void append_run(const ScaledAppend& p, const Places& places, int h, int t, int n, int64_t blk, int off,
                                            float (*red)[4]) {
   const int lane = threadIdx.x & 63, li = lane & 15, sub = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -167,7 +180,7 @@ __device__ __forceinline__ void append_run(const ScaledAppend& p, int h, int t, 
     const int o = o0 + 32 * piece;
     value_rows(y, p, h, t, n, o - off, lane);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) key_row(k[j], p, h, t + min(max(o + 4 * j + sub - off, 0), n - 1), li, kw);
+    for (int j = 0; j < 2; ++j) key_row(k[j], p, places, h, t + min(max(o + 4 * j + sub - off, 0), n - 1), li, kw);
   };
   auto put = [&](const float (&k)[2][8], const bf16x2 (&y)[8], int piece, float kinv, float vinv) {
     const int o = o0 + 32 * piece;
@@ -244,6 +257,7 @@ __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, int rows
     const int64_t s = t >= 0 && t < p.T ? p.slots[t] : -1;
     return s < cap ? s : -1;        // (a slot outside the cache is no slot)
   };
+  const Places places{t0, place_of(p, min(t0 + lane, p.T - 1))};
   const int64_t mine = slot_of(t0 + lane), before = slot_of(t0 + lane - 1);
   const int64_t page = mine < 0 ? 0 : narrow ? (int64_t)((uint32_t)mine / (uint32_t)p.BS) : mine / p.BS;
   const int off = (int)(mine - page * p.BS);
@@ -269,7 +283,7 @@ __device__ __forceinline__ void for_runs(const ScaledAppend& p, int t0, int rows
       n += more == ~0ull ? 64 : __builtin_ctzll(~more);
       if (more != ~0ull) break;
     }
-    run(i, few, t0 + l, n, blk, o);
+    run(i, few, places, t0 + l, n, blk, o);
   }
 }
 
@@ -282,9 +296,9 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = 2 * p.Hkv;
     const int item = b * 4 + w, t = item / per, h = (item - t * per) >> 1;
     if (t >= p.singles) return;
-    for_runs(p, t, 1, [&](int, bool, int t, int n, int64_t blk, int off) {
+    for_runs(p, t, 1, [&](int, bool, const Places& places, int t, int n, int64_t blk, int off) {
       if (item & 1) append_values(p, h, t, n, blk, off);
-      else append_keys(p, h, t, n, blk, off);
+      else append_keys(p, places, h, t, n, blk, off);
     });
     return;
   }
@@ -292,16 +306,17 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(ScaledAppend p, int 
   if (b < run_blocks) {
     const int span = b / p.Hkv, h = b - span * p.Hkv;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for_runs(p, p.singles + rows * span, rows, [&](int i, bool few, int t, int n, int64_t blk, int off) {
+    for_runs(p, p.singles + rows * span, rows, [&](int i, bool few, const Places& places, int t, int n, int64_t blk,
+                                                            int off) {
       if (few) {
-        append_run<HELD>(p, h, t, n, blk, off, red);
+        append_run<HELD>(p, places, h, t, n, blk, off, red);
         return;
       }
       // Many runs, or short ones: a wave to the keys or the values of each.  64 sequences of 3 tokens, 8 kv heads, in
       // spans of 32 rows: 12 us, one run after the other 31; 3 of 2 tokens 5.4, else 10.4.  (Three may be long: 8
       // prompts of ~100 behind 40 11.8 us, by waves 15.8.)
       const int job = 2 * i + (i >> 1);
-      if ((job & 3) == w) append_keys(p, h, t, n, blk, off);
+      if ((job & 3) == w) append_keys(p, places, h, t, n, blk, off);
       if ((job + 1 & 3) == w) append_values(p, h, t, n, blk, off);
     });
     return;

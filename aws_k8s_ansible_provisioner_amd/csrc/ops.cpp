@@ -371,7 +371,8 @@ static void check_angles(const Tensor& qkv, const Tensor& positions, const Tenso
   TORCH_CHECK(positions.scalar_type() == at::kLong && positions.is_contiguous() && positions.numel() >= rows,
               "positions: int64, one per row");
   TORCH_CHECK(cos_sin.scalar_type() == at::kFloat && cos_sin.is_contiguous() && cos_sin.dim() == 2 &&
-                  cos_sin.size(1) == 128 && cos_sin.size(0) > 0 && (uintptr_t)cos_sin.data_ptr() % 16 == 0,
+                  cos_sin.size(1) == 128 && cos_sin.size(0) > 0 && cos_sin.size(0) < (1LL << 31) &&
+                  (uintptr_t)cos_sin.data_ptr() % 16 == 0,
               "cos_sin: contiguous fp32 [max_pos, 128]");
   check_same_device(qkv, {&positions, &cos_sin});
 }
