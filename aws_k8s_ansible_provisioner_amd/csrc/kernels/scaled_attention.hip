@@ -24,14 +24,14 @@ __device__ __forceinline__ int keys_of(const ScaledAttn& p, int seq) {
 }
 
 // ------------------------------------------------------------------------------------------------- decode
-// grid (sequences, kv heads, partitions), four waves that take a partition's 32-token chunks in turn; the columns of
+// grid (sequences, kv heads, partitions), four or eight waves that take a partition's 32-token chunks in turn; the columns of
 // the 16 x 16 x 32 products are the kv head's query heads.  A chunk is 8 loads of 16 bytes to a lane: of K the dims
 // 64 p + 16 g .. + 15 of a token (its k-steps 2 p and 2 p + 1 contract over the first and second 8, q in the same
 // order), of V two dims of an 8-token group.  The next chunk's K is asked for when this one's scores are formed, its
 // V when this one's is used up: a whole chunk on the way in the registers of one.
 // Rows that fill the card are bound by their codes' bytes: 200 rows of up to 4000 keys (16 / 8 heads) 221 us, 6.1 TB/s,
-// 64 of up to 2048 (32 / 8) 35.3, 5.6; few by a chain of loads: one at 333 5.5 us in a graph, 3 of up to 30000 of one kv
-// head 15.8, of which the merge within the launch 3.
+// 64 of up to 2048 (32 / 8) 35.3, 5.6; few by a chain of loads: one at 333 5.1 us in a graph, 3 of up to 30000 of one kv
+// head 13.8, of which the merge within the launch 2 to 3.
 struct Chunk {
   u32x4 k[2][2];   // [16-token tile][p]
   u32x4 v[4];      // dims 32 n + 2 r and + 1 of group g
@@ -126,13 +126,13 @@ __device__ __forceinline__ float part_load(const float* at) {
 }
 
 // The partitions of a (sequence, kv head) into its rows: 16 threads to a row, 8 dims to a thread, 16 / (G rounded
-// up to a power of two) groups of threads that take every so many-th partition, eight of them requested together.
-// lds: 16 rows of D + 4.
-template <bool SHARED>
+// up to a power of two; of eight waves 32) groups of threads that take every so many-th partition, eight of them
+// requested together.  lds: 16 (32) rows of D + 4.
+template <bool SHARED, int NW>
 __device__ __forceinline__ void merge(const ScaledAttn& p, int seq, int kvh, int nparts, int q_tok, float* lds) {
   constexpr int U = 8;
   const int G = p.G, wide = G <= 1 ? 1 : 1 << (32 - __builtin_clz(G - 1));
-  const int at16 = threadIdx.x >> 4, row = at16 & (wide - 1), first = at16 / wide, groups = 16 / wide;
+  const int at16 = threadIdx.x >> 4, row = at16 & (wide - 1), first = at16 / wide, groups = 4 * NW / wide;
   const int d0 = (threadIdx.x & 15) * 8;
   const int64_t base = (int64_t)(seq * p.Hkv + kvh) * p.num_parts * G;
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
@@ -205,7 +205,7 @@ __device__ __forceinline__ void merge(const ScaledAttn& p, int seq, int kvh, int
 __global__ __launch_bounds__(256) void scaled_merge_kernel(ScaledAttn p) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int seq = blockIdx.x, keys = keys_of(p, seq);
-  merge<false>(p, seq, blockIdx.y, min(p.num_parts, (keys + p.part_size - 1) / p.part_size),
+  merge<false, 4>(p, seq, blockIdx.y, min(p.num_parts, (keys + p.part_size - 1) / p.part_size),
                p.q_start ? p.q_start[seq] : seq, lds);
 }
 
@@ -335,14 +335,14 @@ __device__ __forceinline__ void put_v(Chunk& c, const NewKey* key, int tok) {
   }
 }
 
-template <bool FUSED>
-__global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
+template <bool FUSED, int NW>
+__global__ __launch_bounds__(64 * NW, 4) void scaled_decode_kernel(ScaledAttn p) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int seq = blockIdx.x, kvh = blockIdx.y, part = blockIdx.z;
   const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = p.G, BS = p.BS;
-  const int first = part * p.part_size, t0 = first + 32 * w, tok = t0 + 128 * lane;
+  const int first = part * p.part_size, t0 = first + 32 * w, tok = t0 + 32 * NW * lane;
   // page and scales of the wave's chunk `lane` (the host bounds a partition to 64 chunks a wave); the table's entry
   // is asked for beside the length
   const int column = tok / BS;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   const int q_tok = p.q_start ? p.q_start[seq] : seq;
   const int nparts = min(p.num_parts, (keys + p.part_size - 1) / p.part_size);
   if (p.num_parts > 1 && first >= keys) {      // (the merge leaves it out)
-    if (p.tickets != nullptr && part == 0) merge<true>(p, seq, kvh, 0, q_tok, lds);
+    if (p.tickets != nullptr && part == 0) merge<true, NW>(p, seq, kvh, 0, q_tok, lds);
     return;
   }
   NewRow fresh;
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   for (int i = 0; i < 8; ++i) st.o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   st.m = -1e30f;
   st.l = 0.f;
-  for (int t = t0, i = 0; t < end; t += 128, ++i) {
+  for (int t = t0, i = 0; t < end; t += 32 * NW, ++i) {
     const bool some = page_of(i) >= 0;
     float x[8];
     const bool has = FUSED && key != nullptr && (uint32_t)(keys - 1 - t) < 32;
@@ -424,9 +424,9 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   float l = st.l;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  float* o_s = lds;                               // [4][G][D + 4]
-  float* m_s = lds + 4 * G * (D + 4);             // [4][G]
-  float* l_s = m_s + 4 * G;
+  float* o_s = lds;                               // [NW][G][D + 4]
+  float* m_s = lds + NW * G * (D + 4);            // [NW][G]
+  float* l_s = m_s + NW * G;
   if (r < G) {
     float* to = o_s + (w * G + r) * (D + 4) + 8 * g;
 #pragma unroll
@@ -447,9 +447,9 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   if (row < G) {
     float M = -1e30f, L = 0.f, acc[8] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, m_s[i * G + row]);
+    for (int i = 0; i < NW; ++i) M = fmaxf(M, m_s[i * G + row]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NW; ++i) {
       const float f = __builtin_amdgcn_exp2f(m_s[i * G + row] - M);
       L += f * l_s[i * G + row];
 #pragma unroll
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(256, 4) void scaled_decode_kernel(ScaledAttn p) {
   __syncthreads();
   const bool last = *flag != 0;
   __syncthreads();
-  if (last) merge<true>(p, seq, kvh, nparts, q_tok, lds);
+  if (last) merge<true, NW>(p, seq, kvh, nparts, q_tok, lds);
 }
 
 // ------------------------------------------------------------------------------------------------- prompts
@@ -923,27 +923,40 @@ __global__ __launch_bounds__(256) void scaled_prefill_merge_kernel(ScaledAttn p,
 
 void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
   if (num_seqs == 0) return;
-  // Coarser partitions than asked for, in whole ones.  One for up to 512 keys (1 row at 333, 16 / 8 heads, 5.5 us, in two
-  // 7.1), at most 64 (3 rows at ~25000, 8 / 1 heads, 16.2 us, in 118 20.5), else 256 keys or more (1 row at 4000 8.7 us,
-  // 512 10.8); and rows that fill the card by themselves need none, up to 2048 keys (beyond, a long row among short ones
+  // Coarser partitions than asked for, in whole ones.  One for up to 512 keys (1 row at 333, 16 / 8 heads, 5.1 us, in two
+  // 7.0), at most 64 (3 rows at ~25000, 8 / 1 heads, 13.9 us, in 118 19.7), else 256 keys or more (1 row at 4000 8.7 us,
+  // 512 10.3); and rows that fill the card by themselves need none, up to 2048 keys (beyond, a long row among short ones
   // would hold up the step): 64 rows at ~1500 keys of 32 / 8 heads in partitions of 512, 1024, 2048 44, 42, 36 us, 128
-  // at ~1050 65, 60, 53, 16 at ~2250 in 256, 768, 1536 20.6, 18, 22.
+  // at ~1050 65, 60, 53; 16 at ~2250 in 768 and 1024 17.9 and 19.0, 1 at 30000 of 16 / 8 heads in 512 and 768 16.5 and
+  // 17.8 (but 15 at ~5500 of one kv head in 256 and 512 13.2 and 11.8).
   ScaledAttn q = p;
   const int64_t rows = (int64_t)num_seqs * p.Hkv;
-  const int fill = (int)std::min<int64_t>((p.num_parts * rows + 511) / 512, (2047 + p.part_size) / p.part_size);
-  const int by = std::min(std::max({((p.num_parts * p.part_size <= 512 ? 511 : 255) + p.part_size) / p.part_size, (p.num_parts + 63) / 64, fill}),
-                          kDecodeMaxPart / p.part_size);
-  q.part_size = p.part_size * by;
+  const int held = p.num_parts * p.part_size, size = p.part_size;      // (below 2^30)
+  const int fill = (int)std::min<int64_t>((p.num_parts * rows + 511) / 512, (2047 + size) / size);
+  const int least = ((held <= 512 ? 511 : 255) + size) / size;
+  const int by = std::min(std::max({least, (p.num_parts + 63) / 64, fill}), kDecodeMaxPart / size);
+  q.part_size = size * by;
   q.num_parts = (p.num_parts + by - 1) / by;
-  const size_t merging = q.num_parts > 1 ? 16 * (D + 4) : 0;
-  const size_t rows_s = std::max<size_t>(4 * p.G * (D + 4) + 8 * p.G, merging);
+  // Eight waves where a workgroup has a unit to itself and more than a chunk for each: 1 row at 333 5.1 us, by four 5.5,
+  // 16 at ~340 with the append 8.0 and 8.7, 3 at ~25000 13.9 and 16.3; but 1 at 1000 of one kv head, in 256s, 7.9 and 7.1.
+  auto lds = [&](int waves) {
+    return std::max<size_t>(waves * (p.G * (D + 4) + 2 * p.G), q.num_parts > 1 ? 4 * waves * (D + 4) : 0);
+  };
+  const bool wide = rows * q.num_parts <= 256 && std::min(q.part_size, held) > 256 &&
+                    lds(8) * sizeof(float) + sizeof(NewKey) + 16 <= 65536;
+  const size_t rows_s = lds(wide ? 8 : 4);
   q.new_key = (int)(rows_s + 3) / 4 * 4;
   const size_t smem = p.qkv != nullptr ? q.new_key * sizeof(float) + sizeof(NewKey) : rows_s * sizeof(float);
   const dim3 grid(num_seqs, p.Hkv, q.num_parts);
-  if (p.qkv != nullptr) scaled_decode_kernel<true><<<grid, 256, smem, s>>>(q);
-  else scaled_decode_kernel<false><<<grid, 256, smem, s>>>(q);
+  if (p.qkv != nullptr) {
+    if (wide) scaled_decode_kernel<true, 8><<<grid, 512, smem, s>>>(q);
+    else scaled_decode_kernel<true, 4><<<grid, 256, smem, s>>>(q);
+  } else {
+    if (wide) scaled_decode_kernel<false, 8><<<grid, 512, smem, s>>>(q);
+    else scaled_decode_kernel<false, 4><<<grid, 256, smem, s>>>(q);
+  }
   if (q.num_parts > 1 && p.tickets == nullptr)
-    scaled_merge_kernel<<<dim3(num_seqs, p.Hkv), 256, merging * sizeof(float), s>>>(q);
+    scaled_merge_kernel<<<dim3(num_seqs, p.Hkv), 256, 16 * (D + 4) * sizeof(float), s>>>(q);
 }
 
 void launch_scaled_prefill(const ScaledAttn& p, int num_tiles, int tile_rows, int waves, hipStream_t s) {

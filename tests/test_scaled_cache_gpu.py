@@ -184,6 +184,11 @@ def want_rows(c, lens, scale=0.1):
     (2, 2, 32, [3000, 513], 24, 128),
     (16, 2, 32, [700, 40] * 140, 6, 128),                 # rows that fill the card
     (4, 4, 64, [9000], 128, 128),
+    (14, 1, 32, [1000, 400, 0, 33, 520, 1700], 4, 512),    # eight waves, and their merge
+    (1, 1, 32, [5000, 513, 257], 10, 512),
+    (4, 2, 96, [385, 1, 255, 512, 129], 1, 512),
+    (16, 1, 32, [1000, 400, 0, 33], 2, 512),               # too many query heads for eight
+    (16, 8, 32, [300, 700] * 20, 1, 1024),                 # too many rows
 ])
 def test_decode(H, G, page, lens, parts, size):
     c = attention_case(31, H, G, page, lens, [1] * len(lens))
@@ -362,6 +367,9 @@ def step_case(seed, H, G, page, past, norm, room=0):
     (5, 1, 96, [383, 384, 10], True, 2, 384),
     (4, 2, 256, [700, 255, 256, 300, 513], False, 4, 256),
     (15, 1, 32, [40, 64], True, 1, 128),                  # more query heads than one launch takes
+    (14, 1, 32, [700, 5, 1500, 511, 512], True, 4, 512),
+    (4, 2, 64, [1023, 511, 512, 513, 40], False, 2, 1024),
+    (8, 8, 32, [280 + 7 * i for i in range(40)], True, 1, 1024),
 ])
 def test_fused_step(H, G, page, past, norm, parts, size):
     lens, qkv, k, v, s, t, n, pos, sl, cs, w = step_case(51, H, G, page, past, norm)
@@ -382,8 +390,9 @@ def test_fused_step(H, G, page, past, norm, parts, size):
     close(out, want, bound + q_bound(q, entries, t, lens, start, 0.1))
 
 
+@pytest.mark.parametrize("size", [256, 512])            # four waves, eight
 @pytest.mark.parametrize("page", [32, 64, 256])
-def test_fused_step_where_the_scale_grows(page):
+def test_fused_step_where_the_scale_grows(page, size):
     """Every row's key and value are far louder than their page: its codes are rounded anew before they are read,
     whichever chunk of the page a wave holds already."""
     H, G = 4, 2
@@ -393,7 +402,8 @@ def test_fused_step_where_the_scale_grows(page):
     k0, v0, s0 = k.clone(), v.clone(), s.clone()
     k1, v1, s1 = gpu(k, v, s)
     out = torch.empty(len(past), H, D, dtype=torch.bfloat16, device=DEV)
-    ops.scaled_attention_decode_fused(out, *gpu(qkv), k1, v1, s1, *gpu(t, n, pos, sl, cs, *w), H // G, 1e-5, 1e-6)
+    ops.scaled_attention_decode_fused(out, *gpu(qkv), k1, v1, s1, *gpu(t, n, pos, sl, cs, *w), H // G, 1e-5, 1e-6,
+                                      part_size=size)
     check_append(qkv, k0, v0, s0, pos, sl, cs, w, H, G, k1, v1, s1, None)
     assert bool((s1.cpu()[:, sl // page] > s0[:, sl // page]).all())
     q = orc.prepared(qkv, pos, cs, *w, H, G, 1e-6)[0]
