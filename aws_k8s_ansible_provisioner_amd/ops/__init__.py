@@ -335,10 +335,11 @@ def _check_scaled_attention(out, k_cache, v_cache, scales, block_tables, seq_len
         raise RuntimeError("the score scale must be positive")
 
 
-def check_scaled_slots(slots, block_size: int) -> None:
+def check_scaled_slots(slots, block_size: int, num_blocks: Optional[int] = None) -> None:
     """Raise unless a call's rows of one block stand together, in rising slots (what the append kernel
-    takes for granted: a wave owns a block's entries of the call)."""
-    s = [int(x) for x in slots.tolist()]
+    takes for granted: a wave owns a block's entries of the call).  num_blocks: the cache's, where slots behind
+    them are to be no slots, as the append takes them."""
+    s = [x if num_blocks is None or x < num_blocks * block_size else -1 for x in slots.tolist()]
     seen = set()
     for i, x in enumerate(s):
         if x < 0:
@@ -361,7 +362,7 @@ def scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, 
     are); that only divides the work."""
     if _native(qkv):
         if DEBUG_CHECKS:
-            check_scaled_slots(slots[:qkv.shape[0]], k_cache.shape[2])
+            check_scaled_slots(slots[:qkv.shape[0]], k_cache.shape[2], k_cache.shape[0])
         torch.ops.akap.scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin,
                                            q_w, k_w, num_q_heads, num_kv_heads, eps, apply_rope,
                                            qkv.shape[0] if decode else num_decode, q_rows)
@@ -376,7 +377,7 @@ def scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, 
         raise RuntimeError("scaled_cache_append: num_decode / q_rows out of range")
     if positions.dtype != torch.int64 or slots.dtype != torch.int64 or min(positions.numel(), slots.numel()) < T:
         raise RuntimeError("positions / slots: int64, one per row")
-    check_scaled_slots(slots[:T], k_cache.shape[2])
+    check_scaled_slots(slots[:T], k_cache.shape[2], k_cache.shape[0])
     ref.scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin, q_w, k_w,
                             num_q_heads, num_kv_heads, eps, apply_rope, q_rows)
     return q_out

@@ -219,6 +219,20 @@ def test_rows_of_a_block_apart_are_refused():
             ops.check_scaled_slots(torch.tensor(slots), 32)
 
 
+def test_rows_outside_the_cache_are_in_no_block():
+    """Two rows at one slot behind the cache, and rows apart of a block behind it: no entries, and no refusal."""
+    slots = [9999, 40, 41, 9999, 10000, 9998, -5]
+    qkv, k, v, s, pos, sl, cs, w = make(12, 2, 1, len(slots), slots, 32, 3, True)
+    k0, v0, s0 = k.clone(), v.clone(), s.clone()
+    q = torch.empty(len(slots), 2, D, dtype=torch.bfloat16)
+    ops.scaled_cache_append(qkv, q, k, v, s, pos, sl, cs, *w, 2, 1, 1e-6)
+    check_append(qkv, k0, v0, s0, pos, sl, cs, w, 2, 1, k, v, s, q)
+    ops.check_scaled_slots(sl, 32, 3)
+    for bad in ([40, 9999, 41], [40, 40]):
+        with pytest.raises(RuntimeError, match="apart"):
+            ops.check_scaled_slots(torch.tensor(bad), 32, 3)
+
+
 # ------------------------------------------------------------------------------------------------ engine
 def test_engine_on_a_scaled_cache():
     """--kv-cache-dtype fp8_scaled: greedy tokens near the argmax of the dense reference, also where keys are far

@@ -127,6 +127,17 @@ def test_append_rows_that_are_not_finite():
     assert float(s1[1, 1, 0]) >= 2.0 ** -100
 
 
+def test_append_rows_outside_the_cache(monkeypatch):
+    """They are in no block, also for the check of a call's slots."""
+    slots = [9999, 40, 41, 9999, 10000, 9998, -5]
+    case = make(26, 2, 1, len(slots), slots, 32, 3, True)
+    qkv, k, v, s, pos, sl, cs, w = case
+    monkeypatch.setattr(ops, "DEBUG_CHECKS", True)
+    for decode in (False, True):
+        k1, v1, s1, q = run_append(case, 2, 1, slots, decode)
+        check_append(qkv, k, v, s, pos, sl, cs, w, 2, 1, k1, v1, s1, q)
+
+
 def test_append_takes_wide_rows_and_views():
     qkv, k, v, s, pos, sl, cs, w = make(24, 4, 2, 40, list(range(64, 104)), 32, 6, True)
     wide = torch.zeros(40, 8 * D + 64, dtype=torch.bfloat16, device=DEV)
