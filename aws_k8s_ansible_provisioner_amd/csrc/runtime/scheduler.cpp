@@ -450,7 +450,7 @@ void Scheduler::flatten(const std::vector<std::pair<Request*, int>>& sched, Step
     }
     const int kv = start + q;
     buf.seq_lens[s] = kv;
-    info.max_seq_len = std::max(info.max_seq_len, kv);
+    if (!info.is_prefill || (int)s >= info.num_decode) info.max_seq_len = std::max(info.max_seq_len, kv);
     int32_t* row = buf.block_tables + (size_t)s * mb;
     const int nb = (int)r->blocks.size();
     for (int b = 0; b < mb; ++b) row[b] = b < nb ? r->blocks[b] : 0;

@@ -110,7 +110,7 @@ struct StepInfo {
   int num_tokens = 0;
   int num_tiles = 0;
   int num_samples = 0;
-  int max_seq_len = 0;
+  int max_seq_len = 0;  // keys of the longest sequence: of a step with prefill chunks among those
   int num_preempted = 0;
   int num_decode = 0;  // leading single-token decode rows (all rows of a pure decode step)
   int tile_rows = 0;   // prefill tile map granularity of this step

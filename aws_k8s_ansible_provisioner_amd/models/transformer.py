@@ -57,7 +57,7 @@ class AttnBatch:
     tail_slot: Optional[torch.Tensor] = None
     # scaled 8-bit cache: per-layer scales [2, blocks, kv heads]; None = the other caches
     kv_scales: Optional[list] = None
-    max_len: Optional[int] = None  # longest sequence's keys (block tables are wider)
+    max_len: Optional[int] = None  # keys of the prompts' longest sequence (block tables are wider)
 
 
 @dataclasses.dataclass

@@ -463,8 +463,8 @@ def scaled_attention_prefill(out, q, k_cache, v_cache, scales, block_tables, seq
     256; sequences that no tile names are left as they are).
     qprep = (qkv, positions, cos_sin, q_w, eps): the kernel takes its q rows from the projection's, normed and
     rotated by their positions, rounded to bf16 (q is not read then and may be None).
-    max_len: the longest sequence's keys where the host knows them (else what the block tables hold); a map of
-    few tiles over many keys is cut along the keys, by scratch of 520 bytes per row and part."""
+    max_len: the keys of the longest sequence that a tile names, where the host knows them (else what the block
+    tables hold); a map of few tiles over many keys is cut along the keys, by scratch of 520 bytes per row and part."""
     if _native(out):
         waves, parts = scaled_prefill_plan(tile_seq.numel() * k_cache.shape[1], tile_rows,
                                            block_tables.shape[1] * k_cache.shape[2] if max_len is None
