@@ -29,7 +29,8 @@ class EngineConfig:
     chat_template: Optional[str] = None
     kv_role: str = "both"                     # "both" | "prefill" | "decode" (P/D)
     # "auto" (model dtype, bf16) | "fp8" (e4m3fn, scale 1) | "fp8_scaled" (e4m3fn with a power-of-two
-    # scale for each block and kv head: any range of keys and values; one process, no P/D roles)
+    # scale for each block and kv head: any range of keys and values; tensor-parallel ranks keep the
+    # scales of their heads; no P/D roles)
     kv_cache_dtype: str = "auto"
     init_std: float = 0.02                    # random-init weight scale
     shard_init: str = "per_rank"              # "per_rank" | "full" (identical logical weights for any TP)

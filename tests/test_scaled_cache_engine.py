@@ -1,4 +1,9 @@
-"""The engine on the scaled 8-bit cache: mixed steps, entries of any range."""
+"""The engine on the scaled 8-bit cache: mixed steps, entries of any range, tensor parallelism."""
+import json
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -96,3 +101,78 @@ def test_entries_of_any_range_gpu(model, keys, values):
     eng = engine(model, kv_cache_dtype="fp8_scaled", **kw)
     assert eng.runner.graphs
     check_any_range(eng, keys, values, engine(model, kv_cache_dtype="fp8", **kw))
+
+
+# ------------------------------------------------------------------------------------------------ ranks
+CHILD = r"""
+import json, os, sys
+sys.path.insert(0, os.environ["ROOT"])
+from aws_k8s_ansible_provisioner_amd.engine.config import EngineConfig, SamplingParams
+from aws_k8s_ansible_provisioner_amd.parallel import tp_worker
+import torch.distributed as dist
+made = []
+class Runner(tp_worker.ModelRunner):
+    def __init__(self, *a, **kw):
+        super().__init__(*a, **kw)
+        made.append(self)
+tp_worker.ModelRunner = Runner
+ecfg = EngineConfig(model=os.environ["MODEL"], device="cpu", max_model_len=256, max_num_seqs=8,
+                    max_num_batched_tokens=32, block_size=32, num_gpu_blocks=96, kv_cache_dtype="fp8_scaled",
+                    tensor_parallel_size=int(os.environ["WORLD_SIZE"]), shard_init="full", init_std=0.15)
+eng, bc = tp_worker.make_tp_engine(ecfg, backend="gloo", log=lambda *a: None)
+def run(n):
+    return [o.output_ids for o in eng.generate(None, SamplingParams(max_tokens=n, temperature=0, ignore_eos=True),
+                                               prompt_ids=json.loads(os.environ["PROMPTS"]))]
+if eng is not None:
+    if os.environ["TOKENS"] == "1":
+        run(1)
+    else:
+        print("TOKENS " + json.dumps(run(8)), flush=True)
+    bc.shutdown()
+print("SCALES " + json.dumps(made[0].kv_scales[0].log2().tolist()), flush=True)
+"""
+
+
+def ranks(model, world, tokens):
+    """A name -> value lookup of what each rank printed."""
+    from test_tp_cpu import ROOT, _port
+
+    port = _port()
+    procs = [subprocess.Popen([sys.executable, "-c", CHILD], cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.PIPE,
+                              text=True, env=dict(os.environ, RANK=str(r), WORLD_SIZE=str(world), LOCAL_RANK=str(r),
+                                                  MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), ROOT=ROOT,
+                                                  MODEL=model, PROMPTS=json.dumps(PROMPTS), TOKENS=str(tokens),
+                                                  OMP_NUM_THREADS="1"))
+             for r in range(world)]
+    outs = [p.communicate(timeout=300) for p in procs]
+    assert all(p.returncode == 0 for p in procs), [o[1][-3000:] for o in outs]
+    lines = [[x.split(" ", 1) for x in o[0].splitlines() if x.startswith(("TOKENS ", "SCALES "))] for o in outs]
+    return [{name: json.loads(x) for name, x in mine} for mine in lines]
+
+
+MODELS = [("tiny-qwen3", 2), ("tiny-llama", 4)]           # (4 ranks: a kv head on two of them)
+
+
+@pytest.mark.parametrize("model,world", MODELS)
+def test_ranks_answer_as_one_process(model, world):
+    from test_engine_cpu import _near_argmax
+
+    one = _engine(model, kv_cache_dtype="fp8_scaled", shard_init="full")
+    for p, got in zip(PROMPTS, ranks(model, world, 8)[0]["TOKENS"]):
+        assert len(got) == 8
+        _near_argmax(one, p, got, tol=0.5)                # (one process's, in test_scaled_cache)
+
+
+@pytest.mark.parametrize("model,world", MODELS)
+def test_ranks_keep_the_scales_of_their_heads(model, world):
+    """The first layer's keys and values of the prompts are those of one process but for bf16 roundings of the
+    projection, which move a page's largest entry by less than a factor of two: its scale by one power at most."""
+    one = _engine(model, kv_cache_dtype="fp8_scaled", shard_init="full")
+    one.generate(None, SamplingParams(max_tokens=1, **GREEDY), prompt_ids=PROMPTS)
+    whole, hkv = one.runner.kv_scales[0].log2(), one.runner.model.hkv
+    assert bool((whole > -100).any())
+    for rank, said in enumerate(ranks(model, world, 1)):
+        mine = torch.tensor(said["SCALES"])
+        heads = slice(rank * hkv // world, max(rank * hkv // world + 1, (rank + 1) * hkv // world))
+        assert mine.shape == whole[:, :, heads].shape
+        assert bool(((mine - whole[:, :, heads]).abs() <= 1).all())
