@@ -92,6 +92,8 @@ class PDPair:
         IPC handle exchange are made here)."""
         if world < 2:
             raise ValueError("P/D needs at least 2 ranks (prefill + decode)")
+        if getattr(engine.runner, "kv_scales", None) is not None:
+            raise ValueError("P/D moves codes without their scales: no kv_cache_dtype fp8_scaled")
         self.n_prefill, self.n_decode = pd_layout(world, prefill_ranks)
         self.engine = engine
         self.rank, self.world = rank, world

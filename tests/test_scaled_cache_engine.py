@@ -176,3 +176,13 @@ def test_ranks_keep_the_scales_of_their_heads(model, world):
         heads = slice(rank * hkv // world, max(rank * hkv // world + 1, (rank + 1) * hkv // world))
         assert mine.shape == whole[:, :, heads].shape
         assert bool(((mine - whole[:, :, heads]).abs() <= 1).all())
+
+
+def test_pairs_of_prefill_and_decode_are_refused():
+    """Also for engines of no role: what a pair moves would be codes without their scales."""
+    from aws_k8s_ansible_provisioner_amd.parallel.pd_driver import PDPair
+
+    eng = _engine("tiny-qwen3", kv_cache_dtype="fp8_scaled")
+    for rank in range(2):
+        with pytest.raises(ValueError, match="scales"):
+            PDPair(eng, rank, 2)
