@@ -211,6 +211,29 @@ def test_decode(H, G, page, lens, parts, size):
             close(run_decode(c, lens, H, G, parts, size, workspace=ws), *want)
 
 
+# As long as a partition may be: 64 chunks to each of four waves (more query heads than eight take, or more rows), 32 to
+# each of eight.  A sum of 64 chunks takes 8 additions in each, a product's row 32: 2^-13 of the weights' sum of
+# magnitudes beside the 2^-8 of `bound`'s roundings.
+LONG = 1 + 2 ** -4
+
+
+@pytest.mark.parametrize("H,G,page,lens,parts,size", [
+    (16, 1, 32, [8192, 8191, 8161, 8160, 4097, 65], 1, 8192),
+    (2, 2, 32, [8192, 8191, 8161, 4097, 33, 0], 1, 8192),
+    (16, 1, 96, [8064, 8063, 7969, 7968, 4033], 1, 8064),
+    (2, 1, 96, [8064, 8063, 7969, 4033], 1, 8064),
+    (16, 1, 32, [8193, 16384, 8192, 16383, 8224, 100], 2, 8192),
+    (4, 2, 32, [8193, 16384, 8192, 8225], 2, 8192),
+])
+def test_decode_of_whole_partitions(H, G, page, lens, parts, size):
+    c = attention_case(36, H, G, page, lens, [1] * len(lens))
+    want, bound = want_rows(c, lens)
+    close(run_decode(c, lens, H, G, parts, size), want, bound * LONG)
+    if parts > 1:
+        ws = ops.decode_workspace(len(lens), G, H // G, parts, DEV)
+        close(run_decode(c, lens, H, G, parts, size, workspace=ws), want, bound * LONG)
+
+
 def test_decode_beside_codes_that_are_no_numbers():
     """What stands behind a sequence's end, and in other pages, is never seen."""
     lens = [45, 300]
@@ -422,6 +445,33 @@ def test_fused_step_where_the_scale_grows(page, size):
     start = list(range(len(past) + 1))
     want, bound = orc.attention(q, entries, t, lens, start, 1e-5)
     close(out, want, bound + q_bound(q, entries, t, lens, start, 1e-5))
+
+
+@pytest.mark.parametrize("page,size,parts,past", [
+    (32, 8192, 1, [8191, 8190, 8160, 8159, 4096]),
+    (96, 8064, 1, [8063, 8062, 7968, 4032]),
+    (32, 8192, 2, [8192, 16383, 8191, 16350, 8223]),
+    (256, 8192, 1, [8191, 8160, 7937, 8000]),
+])
+@pytest.mark.parametrize("others", [0, 130])             # eight waves, and four
+@pytest.mark.parametrize("loud", [1, 4096])              # (4096: each row's last page is rounded anew)
+def test_fused_step_of_whole_partitions(page, size, parts, past, others, loud):
+    H, G, scale = 4, 2, 0.1 / loud
+    past = past + [i % 70 for i in range(others)]
+    lens, qkv, k, v, s, t, n, pos, sl, cs, w = step_case(58, H, G, page, past, False)
+    qkv[:, H * D:] *= loud
+    k0, v0, s0 = k.clone(), v.clone(), s.clone()
+    k1, v1, s1 = gpu(k, v, s)
+    out = torch.empty(len(past), H, D, dtype=torch.bfloat16, device=DEV)
+    ws = ops.decode_workspace(len(past), G, H // G, parts, DEV)
+    ops.scaled_attention_decode_fused(out, *gpu(qkv), k1, v1, s1, *gpu(t, n, pos, sl, cs, *w), H // G, scale, 1e-6,
+                                      workspace=ws, num_parts=parts, part_size=size)
+    check_append(qkv, k0, v0, s0, pos, sl, cs, w, H, G, k1, v1, s1, None)
+    q = orc.prepared(qkv, pos, cs, *w, H, G, 1e-6)[0]
+    entries = orc.codes(k1, v1) * s1.cpu().double()[..., None, None]
+    start = list(range(len(past) + 1))
+    want, bound = orc.attention(q, entries, t, lens, start, scale)
+    close(out, want, bound * LONG + q_bound(q, entries, t, lens, start, scale))
 
 
 def test_fused_step_of_padding():
