@@ -361,7 +361,7 @@ def scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, 
     (check_scaled_slots).  decode: every row is a single token of its sequence (num_decode: the leading ones
     are); that only divides the work."""
     if _native(qkv):
-        if DEBUG_CHECKS:
+        if DEBUG_CHECKS and not torch.cuda.is_current_stream_capturing():   # (the check copies to the host)
             check_scaled_slots(slots[:qkv.shape[0]], k_cache.shape[2], k_cache.shape[0])
         torch.ops.akap.scaled_cache_append(qkv, q_out, k_cache, v_cache, scales, positions, slots, cos_sin,
                                            q_w, k_w, num_q_heads, num_kv_heads, eps, apply_rope,

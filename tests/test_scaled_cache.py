@@ -233,6 +233,22 @@ def test_rows_outside_the_cache_are_in_no_block():
             ops.check_scaled_slots(torch.tensor(bad), 32, 3)
 
 
+@pytest.mark.parametrize("capturing", [False, True])
+def test_slots_are_not_checked_while_a_graph_is_captured(monkeypatch, capturing):
+    """With AKAP_DEBUG_CHECKS=1 a GPU call copies its slots to the host, which a capture does not survive."""
+    from types import SimpleNamespace as NS
+
+    ran, checked = [], []
+    monkeypatch.setattr(ops, "DEBUG_CHECKS", True)
+    monkeypatch.setattr(ops, "_native", lambda x: True)
+    monkeypatch.setattr(ops, "check_scaled_slots", lambda *a: checked.append(a[1:]))
+    monkeypatch.setattr(ops, "torch", NS(cuda=NS(is_current_stream_capturing=lambda: capturing),
+                                         ops=NS(akap=NS(scaled_cache_append=lambda *a: ran.append(a)))))
+    qkv, k, v, s, pos, sl, cs, w = make(13, 1, 1, 2, [1, 2], 32, 3, False)
+    ops.scaled_cache_append(qkv, qkv, k, v, s, pos, sl, cs, None, None, 1, 1, 1e-6)
+    assert len(ran) == 1 and checked == ([] if capturing else [(32, 3)])
+
+
 # ------------------------------------------------------------------------------------------------ engine
 def test_engine_on_a_scaled_cache():
     """--kv-cache-dtype fp8_scaled: greedy tokens near the argmax of the dense reference, also where keys are far

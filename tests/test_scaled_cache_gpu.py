@@ -593,6 +593,32 @@ def test_step_captured_and_replayed():
             assert torch.equal(a, b)
 
 
+def test_append_captured_with_its_checks(monkeypatch):
+    """AKAP_DEBUG_CHECKS=1 and a captured append: each replay as the eager call."""
+    monkeypatch.setattr(ops, "DEBUG_CHECKS", True)
+    H, G = 4, 2
+    qkv, k, v, s, pos, sl, cs, w = make(72, H, G, 70, list(range(40, 110)), 32, 5, True)
+    x, pos, sl, cs, w0, w1 = gpu(qkv, pos, sl, cs, *w)
+    caches = [gpu(k.clone(), v.clone(), s.clone()) for _ in range(2)]
+    qs = [torch.zeros(70, H, D, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+
+    def append(i):
+        ops.scaled_cache_append(x, qs[i], *caches[i], pos, sl, cs, w0, w1, H, G, 1e-6)
+
+    append(0)
+    append(1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        append(0)
+    for i in range(3):
+        x.mul_(2)
+        graph.replay()
+        append(1)
+        torch.cuda.synchronize()
+        assert torch.equal(*qs) and all(torch.equal(a, b) for a, b in zip(*caches))
+
+
 def test_on_another_stream():
     lens = [400, 33]
     c = attention_case(81, 4, 2, 32, lens, [1, 1])
