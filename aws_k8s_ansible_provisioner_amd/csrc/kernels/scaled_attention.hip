@@ -1,7 +1,10 @@
 // Attention over the scaled 8-bit cache (scaled_cache.h): single rows of running sequences (decode) and rows of
 // prompts.  S^T = K Q^T and O^T = V^T P^T on the matrix cores, keys as rows and queries as columns, so that a
 // query's maximum and sum stay in one lane column; queries and softmax weights are bf16, codes are widened to
-// bf16 with their scale, which is exact, sums and statistics are fp32.
+// bf16 with their scale, which is exact, sums and statistics are fp32.  Weights are rounded because the matrix
+// cores take bf16 at sixteen times the rate of fp32, as the attention over the other caches does it: half a step,
+// 2^-8 of each.  Against 64 bits a step of 128 rows is off by 0.0022 of its outputs' size, with fp32 weights, where
+// the outputs' own rounding is left, by 0.0017.
 //
 // A key is seen if it lies inside the sequence's length, the block table and a page of the cache (a table entry
 // outside the cache: its keys are left out).  A row that sees none is zero.
@@ -552,9 +555,12 @@ __device__ __forceinline__ Tile tile_of(const ScaledAttn& p, int seq, int row0) 
 // laid down one by one (fence): a SIMD issues in order, and a product runs 32 cycles beside the next vector work.
 // Before, with all products of a step and then all weights, and eight waves' later four half a step behind: 1000 behind
 // 9000 in one part, four waves 292 us (now 198), eight 264 (241); 2 of ~759 (20 / 4 heads) 30.5 (23.3); 4 of 4096 (32 /
-// 8) 569 (528).  One wave of 64 rows, whose fragments serve two products: 448 for the 264.
-// Bound by vector work and power: 8 prompts of 2048 (32 / 8 heads) 311 us, 0.88 PFLOP/s, a CU's tile of 256 rows by 64
-// keys in 2.0 us, where the products of a SIMD are 2048 cycles and the vector work of its two waves 2500.
+// 8) 569 (528).  One wave of 64 rows, whose fragments serve two products (tried when a fragment's wait still stood right
+// behind its read): 448 for the 264.
+// Bound by how far products, vector work and LDS run beside each other.  8 prompts of 2048 (32 / 8 heads) 307 us, 0.89
+// PFLOP/s at the 2.2 GHz that the card settles at (lower in the first tens of calls: up to 400 us).  Of a CU's 646 K
+// cycles its matrix units are at work in 43 %, its vector units in 50 %, both together in 21 %, neither in 28 % (a wave
+// waits for LDS, loads or the barrier 30 % of its time); LDS is busy in 33 %, a sixth of that bank conflicts.
 template <int NW>
 __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void scaled_prefill_kernel(ScaledAttn p, int subs) {
   constexpr int ROWS = 32 * NW, NT = 64 * NW, PW = 512 / NT;    // 16-byte pieces of K (and of V) to a thread
@@ -929,6 +935,10 @@ void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
   // would hold up the step): 64 rows at ~1500 keys of 32 / 8 heads in partitions of 512, 1024, 2048 44, 42, 36 us, 128
   // at ~1050 65, 60, 53; 16 at ~2250 in 768 and 1024 17.9 and 19.0, 1 at 30000 of 16 / 8 heads in 512 and 768 16.5 and
   // 17.8 (but 15 at ~5500 of one kv head in 256 and 512 13.2 and 11.8).
+  // All of it goes by the keys that a caller has room for, which in an engine are those of its longest allowed sequence:
+  // short rows there are cut, and take four waves, as long ones would (16 / 8 heads, us, room for the longest row, for
+  // 4096, for 32768 keys: 1 row at 333 5.0, 7.0, 5.4, 1 at 1000 7.8, 7.7, 9.5, 16 at ~340 6.9, 8.1, 8.1, 16 at ~1750 14.2,
+  // 15.8, 22.1; rows that fill the card alike).
   ScaledAttn q = p;
   const int64_t rows = (int64_t)num_seqs * p.Hkv;
   const int held = p.num_parts * p.part_size, size = p.part_size;      // (below 2^30)

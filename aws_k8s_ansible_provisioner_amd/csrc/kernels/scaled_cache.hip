@@ -7,7 +7,7 @@
 // of 8 to 32 rows of the batch for leaders (a wave over one, where rows are single tokens of their sequences) and
 // takes each run: magnitudes first, then the codes.  The caller keeps the rows of a page together, in rising slots.
 // Many rows are bound by their bytes (11881 of 32 / 8 heads 55.6 us, 4.9 TB/s), few by a chain of loads: slots, positions,
-// angles (one row 4.4 us in a graph).
+// angles (one row 3.9 us in a graph).
 #include "scaled_cache.h"
 #include "kernels.h"
 
@@ -330,9 +330,15 @@ void launch_scaled_append(const ScaledAppend& p, hipStream_t s) {
   const long per = 2 * p.Hkv;
   const long single = (p.singles * per + 3) / 4;
   // Runs begin anywhere, and a span's are taken in turn: spans of 8 rows where their workgroups are at most 512, two to a
-  // unit, of 16 up to 1300, else of 32.  8 kv heads, spans of 8, 16 and 32: 49 sequences of 3 tokens 8.2, 12.8 and 20.7
-  // us; 8 of ~130 10.0, 9.0 and 11.8; one of 1000 9.4, 7.7 and 6.9; 40 of ~40 11.5, 11.0 and 12.4; 60 of ~200 46.4, 38.5
-  // and 36.9; 4 kv heads, 24 of ~210 in blocks of 64 14.5, 12.1 and 14.6.
+  // unit, of 16 up to 1300, else of 32.  The shape decides as well, which the host does not know: short and ragged runs
+  // gain by small spans, a prompt that begins its own pages loses (every other span of 16 finds no leader).  8 kv heads,
+  // spans of 8, 16 and 32, us, ten sets of rows in turn or (*) one:
+  //   up to 512     49 sequences of 3 tokens behind some 7.4, 9.9, 15.0; 20 of 24 9.0, 9.4, 12.3; but one of 500 6.2, 5.6, 5.7
+  //   up to 1300    8 of ~130 9.0, 9.8, 10.6; 200 of ~8 13.9, 12.9, 16.0; 4 of ~270 8.6, 8.7, 10.0; 4 of ~585 12.9, 10.1,
+  //                 10.6; but one of 1000 8.0, 6.5, 5.9, of 2048 13.7, 8.4, 7.0; 2 of 1000 12.8, 9.2, 8.6; 4 kv heads, blocks
+  //                 of 64, 24 of ~200 from their pages' first tokens on 15.4, 13.5, 13.1, behind ~30 15.2, 14.1, 14.5
+  //   1340 to 1660  12 of ~220 13.5, 11.9, 12.4; 12 of ~270* 13.6, 13.0, 13.2; 80 of ~40* 17.1, 14.6, 13.8
+  //   from 2000 on  40 of ~100* 17.4, 17.6, 14.7; 20 of ~300* 22.7, 18.7, 17.8; 60 of ~200* 38.3, 28.2, 23.6
   const long rest = p.T - p.singles;
   auto spans = [&](int rows) { return (rest + rows - 1) / rows * p.Hkv; };
   const int rows = spans(8) <= 512 ? 8 : spans(16) <= 1300 ? 16 : 32;
