@@ -937,8 +937,8 @@ void launch_scaled_decode(const ScaledAttn& p, int num_seqs, hipStream_t s) {
   // 17.8 (but 15 at ~5500 of one kv head in 256 and 512 13.2 and 11.8).
   // All of it goes by the keys that a caller has room for, which in an engine are those of its longest allowed sequence:
   // short rows there are cut, and take four waves, as long ones would (16 / 8 heads, us, room for the longest row, for
-  // 4096, for 32768 keys: 1 row at 333 5.0, 7.0, 5.4, 1 at 1000 7.8, 7.7, 9.5, 16 at ~340 6.9, 8.1, 8.1, 16 at ~1750 14.2,
-  // 15.8, 22.1; rows that fill the card alike).
+  // 4096, for 32768 keys: 1 row at 333 5.2, 7.1, 5.6, 1 at 1000 7.8, 7.7, 9.7, 16 at ~340 6.7, 8.0, 8.0, 16 at ~1750 13.0,
+  // 15.9, 22.2; rows that fill the card alike).
   ScaledAttn q = p;
   const int64_t rows = (int64_t)num_seqs * p.Hkv;
   const int held = p.num_parts * p.part_size, size = p.part_size;      // (below 2^30)
