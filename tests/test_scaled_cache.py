@@ -146,6 +146,16 @@ def test_decode_against_64_bits():
     assert not out[1].any()
 
 
+def test_decode_rows_that_q_start_names():
+    lens, rows = [33, 0, 70], torch.tensor([4, 1, 0], dtype=torch.int32)
+    q, k, v, s, t, n, start = attention_case(10, 4, 2, 32, lens, [1] * 3)
+    many, out = torch.zeros(6, 4, D, dtype=torch.bfloat16), torch.full((6, 4, D), 9.0, dtype=torch.bfloat16)
+    many[rows.long()] = q
+    ops.scaled_attention_decode(out, many, k, v, s, t, n, 2, 0.1, q_start=rows)
+    close(out[rows.long()], *orc.attention(q, orc.codes(k, v) * s.double()[..., None, None], t, lens, start, 0.1))
+    assert bool((out[[2, 3, 5]] == 9).all())
+
+
 def test_prompt_against_64_bits():
     lens, new = [40, 64, 5], [40, 3, 5]
     q, k, v, s, t, n, start = attention_case(8, 4, 2, 64, lens, new)
